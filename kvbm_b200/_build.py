@@ -34,12 +34,15 @@ CUDA_SOURCES = [
     CSRC / "kernels" / "kv_xfer.cu",
     CSRC / "kernels" / "kv_multicast.cu",
     CSRC / "kernels" / "llama_ops.cu",
+    CSRC / "kernels" / "batch_tables.cu",
+    CSRC / "kernels" / "kv4_ops.cu",
     CSRC / "kernels" / "kvbm_mem.cu",
     CSRC / "kernels" / "skinny_gemm_tc.cu",
     CSRC / "kernels" / "gds.cpp",
 ]
 CUDA_HEADERS = [CSRC / "kernels" / "common.cuh", CSRC / "kernels" / "kvbm_kernels.h",
-                CSRC / "kernels" / "decode_attn_mma.cuh"]
+                CSRC / "kernels" / "decode_attn_mma.cuh", CSRC / "kernels" / "kv4_format.cuh",
+                CSRC / "kernels" / "paged_decode_kv4.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

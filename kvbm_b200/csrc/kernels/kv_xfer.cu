@@ -691,6 +691,7 @@ int dtype_bytes(int dt) {
     case KVBM_F64:
       return 8;
     case KVBM_FP8_E4M3:
+    case KVBM_U8:
       return 1;
     default:
       return 0;

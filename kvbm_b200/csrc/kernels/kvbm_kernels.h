@@ -21,7 +21,8 @@ extern "C" {
 
 #define KVBM_MAX_LAYERS 128
 
-enum KvbmDtype { KVBM_F16 = 0, KVBM_BF16 = 1, KVBM_F32 = 2, KVBM_F64 = 3, KVBM_FP8_E4M3 = 4 };
+enum KvbmDtype { KVBM_F16 = 0, KVBM_BF16 = 1, KVBM_F32 = 2, KVBM_F64 = 3, KVBM_FP8_E4M3 = 4,
+                 KVBM_U8 = 5 };  // bytes (rows of a 4-bit cache): copied and permuted, never cast
 enum KvbmBlockLayout { KVBM_NHD = 0, KVBM_HND = 1 };
 
 // How one side of a tile transfer turns (pair p, layer i, outer o) into a
@@ -202,6 +203,37 @@ int kvbm_paged_decode_attn_noalloc(const void* q, const void* k_base, const void
                                    float softmax_scale, int splits, void* out, cudaStream_t stream);
 int kvbm_paged_decode_attn_noalloc_max_rows(void);
 const char* kvbm_last_error_message(void);
+
+// ---- block tables and slots (batch_tables.cu) ----
+// Tables, sequence lengths, positions and slots of a batch from its request
+// lengths; `block_counts`, `table`, `rows`, `seq_lens` may be null.
+int kvbm_batch_tables(const int32_t* query_lens, const int32_t* context_lens, const int32_t* block_counts,
+                      const int32_t* block_ids, int64_t num_ids, int batch, int page, int max_blocks, int pad,
+                      int32_t* table, int64_t table_stride, const int32_t* rows, int num_rows, int32_t* seq_lens,
+                      int32_t* cu_query, int32_t* positions, int64_t* slots, int64_t tokens, cudaStream_t stream);
+int kvbm_batch_tables_max_batch(void);
+int kvbm_slot_map(const int32_t* table, int64_t row_stride, int max_blocks, const int32_t* positions, int64_t tokens,
+                  int page, int64_t* slots, cudaStream_t stream);
+
+// ---- 4-bit paged KV cache (kv4_ops.cu; row format in kv4_format.cuh) ----
+// Head norms (optional weights) + RoPE + write into a paged cache, bits = 4 or 16.
+// Without q_out, q and k are rotated in place in qkv; with it qkv stays as it is.
+int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t tokens, int hq, int hkv, int hd, int rot,
+                               const int32_t* positions, const float* cos_sin, int max_pos, const void* q_weight,
+                               const void* k_weight, float eps, int bits, void* kv, int64_t block_stride,
+                               int64_t outer_stride, int64_t token_stride, int64_t head_stride, int page,
+                               int num_blocks, const int64_t* slots, void* q_out, void* k_out, cudaStream_t stream);
+// Rows at `slots` back to bf16, k_out / v_out [tokens, heads, hd]; a slot outside the pool gives zeros.
+int kvbm_kv4_gather(const void* kv, int64_t block_stride, int64_t outer_stride, int64_t token_stride,
+                    int64_t head_stride, int page, int num_blocks, int heads, int hd, const int64_t* slots,
+                    int64_t tokens, void* k_out, void* v_out, cudaStream_t stream);
+// Decode attention over the 4-bit cache; q and out [batch, hq, hd] bf16.
+int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const void* kv, int64_t block_stride,
+                               int64_t outer_stride, int64_t token_stride, int64_t head_stride, int page,
+                               int num_blocks, const int32_t* block_table, int64_t table_stride, int max_blocks,
+                               const int32_t* seq_lens, int batch, int hq, int hkv, int hd, float softmax_scale,
+                               int splits, float* part_acc, float* part_ml, unsigned int* counters, void* out,
+                               cudaStream_t stream);
 
 #ifdef __cplusplus
 }

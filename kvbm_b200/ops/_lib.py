@@ -14,7 +14,7 @@ from .. import _build
 
 MAX_LAYERS = 128
 
-F16, BF16, F32, F64, FP8_E4M3 = 0, 1, 2, 3, 4
+F16, BF16, F32, F64, FP8_E4M3, U8 = 0, 1, 2, 3, 4, 5
 NHD, HND = 0, 1
 ADDR_LAYER_BASES, ADDR_BLOCK_TABLE, ADDR_CHUNK_TABLE = 0, 1, 2
 
@@ -125,6 +125,26 @@ _SIGS = {
         [_VP, _VP, _VP, _I64, _I64, _I64, _INT, _VP, _INT, _VP, _INT, _INT, _INT, _INT, _F32, _INT, _VP, _VP, _VP,
          _VP],
     ),
+    "kvbm_batch_tables": (
+        _INT,
+        [_VP, _VP, _VP, _VP, _I64, _INT, _INT, _INT, _INT, _VP, _I64, _VP, _INT, _VP, _VP, _VP, _VP, _I64, _VP],
+    ),
+    "kvbm_batch_tables_max_batch": (_INT, []),
+    "kvbm_slot_map": (_INT, [_VP, _I64, _INT, _VP, _I64, _INT, _VP, _VP]),
+    "kvbm_qk_norm_rope_kv_write": (
+        _INT,
+        [_VP, _I64, _I64, _INT, _INT, _INT, _INT, _VP, _VP, _INT, _VP, _VP, _F32, _INT, _VP, _I64, _I64, _I64, _I64,
+         _INT, _INT, _VP, _VP, _VP, _VP],
+    ),
+    "kvbm_kv4_gather": (
+        _INT,
+        [_VP, _I64, _I64, _I64, _I64, _INT, _INT, _INT, _INT, _VP, _I64, _VP, _VP, _VP],
+    ),
+    "kvbm_paged_decode_attn_kv4": (
+        _INT,
+        [_VP, _I64, _VP, _I64, _I64, _I64, _I64, _INT, _INT, _VP, _I64, _INT, _VP, _INT, _INT, _INT, _INT, _F32, _INT,
+         _VP, _VP, _VP, _VP, _VP],
+    ),
     "kvbm_skinny_gemm": (_INT, [_VP, _INT, _VP, _INT, _VP, _INT, _INT, _INT, _INT, _INT, _VP, _VP, _VP]),
     "kvbm_skinny_gemm_ctas": (_INT, []),
     "kvbm_skinny_gemm_set_pdl": (_INT, [_INT]),
@@ -172,6 +192,8 @@ _KERNELS_PER_CALL = {
     "kvbm_signal_flag_payload": 1, "kvbm_wait_flags_all": 1, "kvbm_rmsnorm": 1, "kvbm_rope_kv_write": 1,
     "kvbm_rope_kv_push": 1, "kvbm_rope_kv_write_qout": 1, "kvbm_rope_kv_push_heads": 1,
     "kvbm_silu_mul": 1, "kvbm_paged_decode_attn": 2, "kvbm_paged_decode_attn_fused": 1, "kvbm_paged_decode_attn_simt": 2,
+    "kvbm_batch_tables": 1, "kvbm_slot_map": 1, "kvbm_qk_norm_rope_kv_write": 1, "kvbm_kv4_gather": 1,
+    "kvbm_paged_decode_attn_kv4": 1,
     "kvbm_skinny_gemm": 1, "kvbm_kv_multicast": 1, "kvbm_signal_multicast": 1,
 }
 _launches = 0
@@ -221,3 +243,43 @@ def check(code: int, what: str = "") -> None:
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
     count_launches(_KERNELS_PER_CALL.get(name, 0))
+
+
+class on_device:
+    """Makes ``device`` current and, given a stream (``torch.cuda.Stream`` or handle), that stream: what is
+    allocated inside belongs to the stream the kernel runs on. Yields the stream's handle."""
+
+    __slots__ = ("_dev", "_stream", "_prev", "_ctx")
+
+    def __init__(self, device, stream=None):
+        import torch
+
+        if device.type != "cuda":
+            raise ValueError(f"the kernels take CUDA tensors, not tensors on {device}")
+        if stream is not None and not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=device)
+        if stream is not None and stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        self._dev, self._stream, self._ctx, self._prev = device, stream, None, -1
+
+    def __enter__(self) -> int:
+        import torch
+
+        cur = torch.cuda.current_device()
+        if self._dev.index != cur:
+            self._prev = cur
+            torch.cuda.set_device(self._dev.index)
+        s = self._stream
+        if s is None:
+            return torch.cuda.current_stream().cuda_stream
+        self._ctx = torch.cuda.stream(s)
+        self._ctx.__enter__()
+        return s.cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        import torch
+
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+        if self._prev >= 0:
+            torch.cuda.set_device(self._prev)

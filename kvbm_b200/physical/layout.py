@@ -38,6 +38,7 @@ DTYPE_CODE = {
     torch.float32: _lib.F32,
     torch.float64: _lib.F64,
     torch.float8_e4m3fn: _lib.FP8_E4M3,
+    torch.uint8: _lib.U8,
 }
 DTYPE_NAME = {
     torch.float16: "float16",
@@ -45,6 +46,7 @@ DTYPE_NAME = {
     torch.float32: "float32",
     torch.float64: "float64",
     torch.float8_e4m3fn: "float8_e4m3fn",
+    torch.uint8: "uint8",  # rows of bytes (a 4-bit cache): copied and permuted, never cast
 }
 NAME_DTYPE = {v: k for k, v in DTYPE_NAME.items()}
 

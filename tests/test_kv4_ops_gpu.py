@@ -1,0 +1,530 @@
+"""GPU numerics of the 4-bit cache's operators against plain forms in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from kvbm_b200.ops import kv4_ops, table_ops
+from kvbm_b200.physical.layout import KvBlockLayout, KvLayout, LayoutConfig
+
+BF = torch.bfloat16
+HALF_STEP = 2.0 ** -8  # of a bf16, relative
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _empty_pool(nb, page, heads, hd, bits=4, order="nhd", fill=0):
+    width, dtype = (kv4_ops.row_bytes(hd), torch.uint8) if bits == 4 else (hd, BF)
+    if order == "hnd":
+        return torch.full((nb, 2, heads, page, width), fill, dtype=dtype, device="cuda").transpose(2, 3)
+    return torch.full((nb, 2, page, heads, width), fill, dtype=dtype, device="cuda")
+
+
+# ------------------------------------------------------------------ tables
+
+
+def _plain_tables(q, c, ids, page, max_blocks, T, counts=None, pad=0):
+    table, seq, cu, pos, slots = [], [], [0], [], []
+    at = 0
+    for b in range(len(q)):
+        qb, cb = max(q[b], 0), max(c[b], 0)
+        n = max(counts[b], 0) if counts is not None else -(-(qb + cb) // page)
+        mine = ids[at: at + n][:max_blocks]
+        at += n
+        table.append(mine + [pad] * (max_blocks - len(mine)))
+        seq.append(qb + cb)
+        cu.append(cu[-1] + qb)
+        for p in range(cb, cb + qb):
+            pos.append(p)
+            ok = p // page < len(mine) and mine[p // page] >= 0
+            slots.append(mine[p // page] * page + p % page if ok else -1)
+    pos, slots = pos[:T], slots[:T]
+    return table, seq, cu, pos + [0] * (T - len(pos)), slots + [-1] * (T - len(slots))
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("q,c,page,max_blocks,T,counts,n_ids", [
+    ([], [], 16, 4, 5, None, 0),                              # no request at all
+    ([1], [0], 16, 1, 1, None, 1),
+    ([0, 0, 3], [0, 33, 0], 16, 4, 7, None, 4),               # nothing new, an empty one, a padded batch
+    ([5, -2, 17], [-4, 16, 15], 16, 3, 22, None, 5),          # negative lengths count as 0
+    ([40, 9], [100, 3], 16, 4, 49, None, 20),                 # 9 blocks needed, a table of 4
+    ([40, 9], [100, 3], 16, 16, 20, None, 20),                # fewer places than tokens
+    ([4, 4, 4], [60, 0, 12], 16, 8, 12, [2, 5, 1], 8),        # reserved ahead, and too few
+    ([4, 4, 4], [60, 0, 12], 1, 70, 12, None, 70),            # ids run out
+    ([7] * 300, list(range(300)), 32, 12, 2200, None, 3000),  # more requests than threads
+    ([3000, 1, 1], [1, 5000, 0], 128, 64, 3002, None, 80),
+])
+def test_batch_tables(q, c, page, max_blocks, T, counts, n_ids):
+    ids = torch.randperm(max(n_ids, 1), generator=torch.Generator().manual_seed(n_ids))[:n_ids].tolist()
+    if n_ids > 3:
+        ids[2] = -1  # a block that is not there
+    got = table_ops.batch_tables(_i32(q), _i32(c), _i32(ids), page=page, max_blocks=max_blocks, num_tokens=T,
+                                 block_counts=_i32(counts) if counts else None, pad_block=9)
+    want = _plain_tables(q, c, ids, page, max_blocks, T, counts, pad=9)
+    for g, w, name in zip(got, want, got._fields):
+        assert g.tolist() == w, name
+
+
+def test_batch_tables_into_rows_of_a_persistent_table():
+    table = torch.full((6, 8), -7, dtype=torch.int32, device="cuda")[:, :5]  # strided rows
+    got = table_ops.batch_tables(_i32([1, 2, 1]), _i32([16, 0, 3]), _i32([4, 5, 6, 7]), page=16, num_tokens=4,
+                                 table=table, rows=_i32([4, 1, 99]), pad_block=2)
+    assert got.block_table.data_ptr() == table.data_ptr()
+    assert table.tolist() == [[-7] * 5, [6, 2, 2, 2, 2], [-7] * 5, [-7] * 5, [4, 5, 2, 2, 2], [-7] * 5]
+    assert got.slots.tolist() == [80, 96, 97, 115]
+
+
+@pytest.mark.parametrize("B", [1, 256, 8192])
+def test_batch_tables_largest_batches(B):
+    g = torch.Generator().manual_seed(B)
+    q = torch.randint(0, 3, (B,), generator=g).tolist()
+    c = torch.randint(0, 40, (B,), generator=g).tolist()
+    n = sum(-(-(a + b) // 16) for a, b in zip(q, c))
+    ids = torch.randperm(n + 1, generator=g)[:n].tolist()
+    got = table_ops.batch_tables(_i32(q), _i32(c), _i32(ids), page=16, max_blocks=3, num_tokens=sum(q) + 3)
+    for a, w in zip(got, _plain_tables(q, c, ids, 16, 3, sum(q) + 3)):
+        assert a.tolist() == w
+
+
+@pytest.mark.parametrize("page", [1, 16, 64])
+def test_slot_map(page):
+    table = torch.randperm(7 * 9, generator=torch.Generator().manual_seed(page)).int().view(7, 9).cuda()
+    table[2, 0] = -1
+    pos = _i32([0, 5 * page, 0, 9 * page, -1, 9 * page - 1, 2 ** 31 - 1])
+    want = [int(table[i, p // page]) * page + p % page if 0 <= p < 9 * page and int(table[i, p // page]) >= 0 else -1
+            for i, p in enumerate(pos.tolist())]
+    assert table_ops.slot_map(table, pos, page=page).tolist() == want
+    one = table_ops.slot_map(table[3], torch.arange(9 * page, dtype=torch.int32, device="cuda"), page=page)
+    assert one.tolist() == [int(table[3, p // page]) * page + p % page for p in range(9 * page)]
+    wide = torch.zeros(7, 20, dtype=torch.int32, device="cuda")
+    wide[:, :9] = table
+    assert table_ops.slot_map(wide[:, :9], pos, page=page).tolist() == want
+    assert table_ops.slot_map(table[:0], pos[:0], page=page).numel() == 0
+
+
+# ------------------------------------------------------------------- write
+
+
+def _cos_sin(n, rot):
+    inv = 500000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    f = torch.outer(torch.arange(n, dtype=torch.float64), inv)
+    return torch.cat([f.cos(), f.sin()], -1).float().cuda()
+
+
+def _heads64(qkv, pos, cs, hq, hkv, qw, kw, eps):
+    """Normalised and rotated q and k in 64 bits, and the size the rotation's rounding is relative to."""
+    rot = cs.shape[1]
+    x = qkv.double()
+    c, s = cs.double()[pos.long()][:, None, : rot // 2], cs.double()[pos.long()][:, None, rot // 2:]
+
+    def turn(y, w):
+        if w is not None:
+            y = y / (y.pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+        a, b = y[..., : rot // 2], y[..., rot // 2: rot]
+        out = torch.cat([a * c - b * s, b * c + a * s, y[..., rot:]], -1)
+        size = torch.cat([(a * c).abs() + (b * s).abs(), (b * c).abs() + (a * s).abs(), y[..., rot:].abs()], -1)
+        return out, size
+
+    return turn(x[:, :hq], qw), turn(x[:, hq: hq + hkv], kw)
+
+
+def _close(got, want, size):
+    # one rounding to bf16, after about a dozen in fp32 relative to the terms' sizes (128 squares summed in a
+    # tree of 3 + log2 steps, a root, a quotient, two products and a sum): below 2^-19 of them
+    err = (got.double() - want).abs()
+    assert (err <= HALF_STEP * want.abs() + 2.0 ** -19 * size + 2.0 ** -133).all(), float(err.max())
+
+
+@pytest.mark.parametrize("T,hq,hkv,hd,rot,page,bits,order,norm,out", [
+    (1, 32, 8, 128, 128, 16, 4, "nhd", True, "q"),
+    (50, 8, 2, 128, 128, 16, 4, "hnd", True, None),
+    (33, 5, 1, 64, 32, 32, 4, "nhd", True, "qk"),
+    (19, 3, 3, 256, 256, 1, 4, "hnd", True, "qk"),
+    (70, 7, 3, 128, 48, 64, 16, "hnd", True, "qk"),
+    (21, 4, 2, 256, 128, 16, 16, "nhd", "k", None),
+    (9, 0, 4, 64, 64, 16, 4, "nhd", "q", None),
+    (300, 12, 2, 128, 128, 16, 4, "nhd", False, "q"),
+    (17, 1, 1, 64, 16, 16, 16, "nhd", True, None),
+])
+def test_qk_norm_rope_kv_write(T, hq, hkv, hd, rot, page, bits, order, norm, out):
+    g = _gen(T * hd)
+    nb = -(-T // page) + 2
+    kv = _empty_pool(nb, page, hkv, hd, bits, order, fill=3)
+    before = kv.clone()
+    wide = torch.randn(T, (hq + 2 * hkv) * hd + 24, device="cuda", generator=g).to(BF)  # rows with a gap behind them
+    qkv = wide[:, : (hq + 2 * hkv) * hd].view(T, hq + 2 * hkv, hd)
+    orig = wide.clone()
+    pos = torch.randint(0, 500, (T,), device="cuda", generator=g).int()
+    slots = torch.randperm(nb * page, device="cuda", generator=g)[:T]
+    cs = _cos_sin(500, rot)
+    qw = (1 + 0.3 * torch.randn(hd, device="cuda", generator=g)).to(BF) if norm in (True, "q") else None
+    kw = (1 + 0.3 * torch.randn(hd, device="cuda", generator=g)).to(BF) if norm in (True, "k") else None
+    if T > 8:
+        pos[3] = 500      # outside the table: left alone
+        pos[4] = -1
+        slots[5] = -1     # not written
+        slots[6] = nb * page
+    o = orig[:, : (hq + 2 * hkv) * hd].view(T, hq + 2 * hkv, hd)
+    (q64, q_size), (k64, k_size) = _heads64(o, pos.clamp(0, 499), cs, hq, hkv, qw, kw, 1e-6)
+    q_out = torch.full((T, hq, hd), 5.0, device="cuda", dtype=BF) if out else None
+    k_out = torch.full((T, hkv, hd), 5.0, device="cuda", dtype=BF) if out == "qk" else None
+    kv4_ops.qk_norm_rope_kv_write(qkv, pos, cs, hq, hkv, kv, slots, q_weight=qw, k_weight=kw, eps=1e-6, q_out=q_out,
+                                  k_out=k_out)
+    torch.cuda.synchronize()
+    live = torch.ones(T, dtype=torch.bool, device="cuda")
+    if T > 8:
+        live[3:5] = False
+    if out:
+        assert torch.equal(wide, orig)
+        assert (q_out[~live] == 5).all() and (k_out is None or (k_out[~live] == 5).all())
+        q, k = q_out, k_out
+    else:
+        assert torch.equal(wide[:, (hq + 2 * hkv) * hd:], orig[:, (hq + 2 * hkv) * hd:])
+        assert torch.equal(qkv[:, hq + hkv:], o[:, hq + hkv:]) and torch.equal(qkv[~live], o[~live])
+        q, k = qkv[:, :hq], qkv[:, hq: hq + hkv]
+    _close(q[live], q64[live], q_size[live])
+    if k is not None:
+        _close(k[live], k64[live], k_size[live])
+    stored = live.clone()
+    if T > 8:
+        stored[5:7] = False
+    s = slots[stored]
+    touched = torch.zeros(nb, page, dtype=torch.bool, device="cuda")
+    touched[s // page, s % page] = True
+    keep = ~touched[:, None, :, None, None].expand_as(kv)
+    assert torch.equal(kv[keep], before[keep])  # every other row is as it was
+    rows_k, rows_v = kv[s // page, 0, s % page], kv[s // page, 1, s % page]
+    v = o[stored][:, hq + hkv:]
+    if bits == 16:
+        assert torch.equal(rows_v, v)
+        _close(rows_k, k64[stored], k_size[stored])
+        assert k is None or torch.equal(rows_k, k[stored])
+    else:
+        assert torch.equal(rows_v, kv4_ops.pack_rows(v, True))
+        if k is not None:
+            assert torch.equal(rows_k, kv4_ops.pack_rows(k[stored], False))
+        else:
+            back = kv4_ops.unpack_rows(rows_k, False).double()
+            span = (k64[stored].unflatten(-1, (-1, 32)).amax(-1) - k64[stored].unflatten(-1, (-1, 32)).amin(-1))
+            # half a step of the rounded-up scale, and the bf16 rounding of the element and of the range's ends
+            bound = span / 30 * (1 + 2.0 ** -7) + 2.0 ** -7 * k64[stored].unflatten(-1, (-1, 32)).abs().amax(-1)
+            err = (back - k64[stored]).abs().unflatten(-1, (-1, 32)).amax(-1)
+            assert (err <= bound).all()
+
+
+def test_write_poisoned_and_constant_groups():
+    hkv, hd, page = 2, 128, 16
+    kv = _empty_pool(2, page, hkv, hd)
+    x = torch.randn(8, 3 * hkv, hd, device="cuda", generator=_gen(1)).to(BF)
+    x[0, 4, 3], x[1, 5, 40], x[2, 4, 127] = math.inf, math.nan, -math.inf
+    x[3, 4] = 0.75
+    x[4, 4] = 0.0
+    x[5, 4, :32] = torch.linspace(-1, 1, 32).to(BF) * 1e38
+    x[6, 4] = torch.finfo(BF).tiny / 4
+    kv4_ops.qk_norm_rope_kv_write(x.clone(), torch.zeros(8, dtype=torch.int32, device="cuda"), _cos_sin(1, hd), hkv, hkv,
+                                  kv, torch.arange(8, device="cuda"))
+    assert torch.equal(kv[0, 1, :8], kv4_ops.pack_rows(x[:, 2 * hkv:], True))
+    k, v = kv4_ops.kv4_gather(kv, torch.arange(8, device="cuda"))
+    assert v[0, 0, :32].isnan().all() and v[0, 0, 32:].isfinite().all()
+    assert torch.equal(v[3, 0], x[3, 4]) and torch.equal(v[4, 0], x[4, 4]) and torch.equal(v[6, 0], x[6, 4])
+
+
+@pytest.mark.parametrize("order", ["nhd", "hnd"])
+@pytest.mark.parametrize("T,heads,hd,page", [(0, 2, 64, 16), (1, 1, 64, 1), (77, 8, 128, 16), (130, 3, 256, 32)])
+def test_gather(T, heads, hd, page, order):
+    nb = -(-T // page) + 1
+    kv = _empty_pool(nb, page, heads, hd, order=order)
+    x = torch.randn(nb, 2, page, heads, hd, device="cuda", generator=_gen(T)).to(BF)
+    kv[:, 0], kv[:, 1] = kv4_ops.pack_rows(x[:, 0], False), kv4_ops.pack_rows(x[:, 1], True)
+    slots = torch.randint(0, nb * page, (T,), device="cuda", generator=_gen(T + 1))  # repeats allowed
+    if T > 3:
+        slots[1], slots[2] = -1, nb * page
+    k, v = kv4_ops.kv4_gather(kv, slots)
+    ok = (slots >= 0) & (slots < nb * page)
+    s = slots[ok]
+    for got, o in ((k, 0), (v, 1)):
+        rows = kv[s // page, o, s % page]
+        assert torch.equal(got[ok], kv4_ops.unpack_rows(rows, bool(o)).to(BF))
+        assert not got[~ok].any() and got.shape == (T, heads, hd)
+
+
+# --------------------------------------------------------------- attention
+
+
+def _filled(B, lens, heads, hd, page, order="nhd", seed=0, spread=1.0):
+    """A pool whose live rows hold data and all others 0xff, its table, and the values in 64 bits."""
+    nb = max(1, -(-max(max(lens), 1) // page))
+    kv = _empty_pool(B * nb + 2, page, heads, hd, order=order, fill=255)
+    g = _gen(seed)
+    table = (torch.randperm(B * nb, device="cuda", generator=g) + 2).int().view(B, nb)
+    x = torch.randn(B, nb * page, 2, heads, hd, device="cuda", generator=g)
+    x[..., 5] *= 4 * spread
+    x[:, :, 1] += 0.3
+    x = x.to(BF)
+    vals = []
+    for b in range(B):
+        rk, rv = kv4_ops.pack_rows(x[b, :, 0], False), kv4_ops.pack_rows(x[b, :, 1], True)
+        for j in range(-(-lens[b] // page)):
+            n = min(page, lens[b] - j * page)
+            kv[int(table[b, j]), 0, :n] = rk[j * page: j * page + n]
+            kv[int(table[b, j]), 1, :n] = rv[j * page: j * page + n]
+        vals.append((kv4_ops.unpack_rows(rk[: lens[b]], False).double(), kv4_ops.unpack_rows(rv[: lens[b]], True).double()))
+    return kv, table, vals
+
+
+def _attn64(q, vals, scale):
+    B, hq, hd = q.shape
+    out, size = torch.zeros(2, B, hq, hd, dtype=torch.float64, device="cuda")
+    for b, (k, v) in enumerate(vals):
+        if k.shape[0]:
+            rep = hq // k.shape[1]
+            kk, vv = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+            p = torch.softmax(torch.einsum("hd,nhd->hn", q[b].double(), kk) * scale, -1)
+            out[b] = torch.einsum("hn,nhd->hd", p, vv)
+            size[b] = torch.einsum("hn,nhd->hd", p, vv.abs())
+    return out, size
+
+
+def _check_attn(got, q, vals, scale, **kw):
+    want, size = _attn64(q, vals, scale)
+    # one rounding of the result to bf16 and one of each weight p (relative 2^-8 each, so of sum p |v|); scores
+    # carry fp32 rounding of |scale q . k| terms, far below: another 2^-10 of sum p |v|
+    bound = HALF_STEP * want.abs() + (HALF_STEP + 2.0 ** -10) * size + 1e-30
+    err = (got.double() - want).abs()
+    assert (err <= bound).all(), (float((err - bound).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("counters", [False, True])
+@pytest.mark.parametrize("lens,hkv,group,hd,page,order,splits", [
+    ([1], 1, 1, 64, 16, "nhd", None),
+    ([1, 2, 15, 16, 17, 31, 33], 2, 4, 128, 16, "nhd", 1),
+    ([0, 300, 5, 64, 65], 2, 7, 64, 32, "hnd", 3),           # an empty request
+    ([0, 0], 1, 3, 128, 16, "nhd", 2),                        # nothing but empty ones
+    ([129, 1000], 3, 5, 128, 64, "hnd", None),
+    ([77, 700, 3], 1, 8, 256, 16, "nhd", 5),
+    ([40, 41], 2, 1, 256, 1, "nhd", 2),                       # pages of one token
+    ([100, 513], 2, 2, 128, 8, "hnd", 4),                     # pages that end inside a tile
+    ([257, 90], 1, 16, 64, 16, "nhd", 3),                     # more query heads than a CTA takes
+    ([333, 47], 1, 13, 128, 16, "hnd", 7),
+    ([2100], 8, 4, 128, 16, "nhd", 40),                       # more ranges than pages for some
+    ([5], 4, 6, 64, 128, "nhd", 9),
+])
+def test_paged_decode_attention(lens, hkv, group, hd, page, order, splits, counters):
+    B = len(lens)
+    kv, table, vals = _filled(B, lens, hkv, hd, page, order, seed=sum(lens) + hd)
+    q = 2 * torch.randn(B, hkv * group, hd, device="cuda", generator=_gen(9))
+    q = q.to(BF)
+    c = torch.zeros(B * hkv * group, dtype=torch.int32, device="cuda") if counters else None
+    seq = _i32(lens)
+    for _ in range(2):  # the tickets are left zero
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 1 / math.sqrt(hd), splits=splits, counters=c)
+        _check_attn(got, q, vals, 1 / math.sqrt(hd))
+        assert c is None or not c.any()
+    for b, n in enumerate(lens):
+        assert n or not got[b].any()
+
+
+def test_attention_strided_query_table_and_caller_buffers():
+    lens, hkv, group, hd, page = [90, 200, 17], 2, 4, 128, 16
+    kv, table, vals = _filled(3, lens, hkv, hd, page, seed=4)
+    wide = torch.randn(3, 8 + 2 * hkv, hd, device="cuda", generator=_gen(1)).to(BF)
+    q = wide[:, :8]
+    big = torch.zeros(3, table.shape[1] + 5, dtype=torch.int32, device="cuda")
+    big[:, : table.shape[1]] = table
+    scratch = torch.full((3 * 8 * 4 * (hd + 2),), math.nan, device="cuda")
+    out = torch.empty(3, 8, hd, dtype=BF, device="cuda")
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, big[:, : table.shape[1]], _i32(lens), 0.1, splits=4, scratch=scratch, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    _check_attn(got, q, vals, 0.1)
+    # a table wider than the sequences need, and lengths beyond the table's width
+    _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, big, _i32(lens), 0.1), q, vals, 0.1)
+    full = table[:, :1].contiguous()
+    vals1 = [(k[:16], v[:16]) for k, v in vals]
+    _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, full, _i32([90, 2 ** 31 - 1, 17]), 0.1), q, vals1, 0.1)
+    none = kv4_ops.paged_decode_attn_kv4(q, kv, table[:, :0], _i32(lens), 0.1)
+    assert not none.any()
+    assert kv4_ops.paged_decode_attn_kv4(q[:0], kv, table[:0], _i32([]), 0.1).shape == (0, 8, hd)
+
+
+def test_attention_pages_outside_the_pool_hold_no_tokens():
+    lens, hkv, hd, page = [64, 64, 64], 2, 128, 16
+    kv, table, vals = _filled(3, lens, hkv, hd, page, seed=6)
+    table[0, 1], table[1, 0], table[2] = -1, kv.shape[0], 2 ** 30
+    keep = [torch.arange(64, device="cuda") // 16 != 1, torch.arange(64, device="cuda") // 16 != 0,
+            torch.zeros(64, dtype=torch.bool, device="cuda")]
+    q = torch.randn(3, 8, hd, device="cuda", generator=_gen(2)).to(BF)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.2, splits=2)
+    _check_attn(got, q, [(k[m], v[m]) for (k, v), m in zip(vals, keep)], 0.2)
+    assert not got[2].any()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-4, 3.0, -0.5])
+def test_attention_scales(scale):
+    """Equal weights, and weights that sit on one token; q elements of very different size."""
+    lens, hkv, group, hd = [200, 33], 1, 4, 128
+    kv, table, vals = _filled(2, lens, hkv, hd, 16, seed=8)
+    q = (torch.randn(2, 4, hd, device="cuda", generator=_gen(3)) *
+         torch.logspace(-4, 0, hd, device="cuda")).to(BF)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), scale)
+    _check_attn(got, q, vals, scale)
+
+
+def test_attention_one_token_far_above_many():
+    """A first token of almost all weight in front of many of little: their sum still counts."""
+    n, hd = 4096, 64
+    kv, table, _ = _filled(1, [n], 1, hd, 16, seed=10)
+    x = torch.zeros(n, 2, 1, hd, device="cuda")
+    x[0, 0, 0, 0], x[1:, 1] = 8.0, 1.0
+    x[0, 1] = -1.0
+    x = x.to(BF)
+    rk, rv = kv4_ops.pack_rows(x[:, 0], False), kv4_ops.pack_rows(x[:, 1], True)
+    for j in range(n // 16):
+        kv[int(table[0, j]), 0], kv[int(table[0, j]), 1] = rk[16 * j: 16 * j + 16], rv[16 * j: 16 * j + 16]
+    q = torch.zeros(1, 1, hd, device="cuda", dtype=BF)
+    q[0, 0, 0] = 1.0
+    vals = [(kv4_ops.unpack_rows(rk, False).double(), kv4_ops.unpack_rows(rv, True).double())]
+    for splits in (1, 8):
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, splits=splits)
+        _check_attn(got, q, vals, 1.0)
+
+
+def test_attention_poison_shows_only_where_it_is():
+    lens, hkv, hd = [40, 40], 2, 128
+    kv, table, vals = _filled(2, lens, hkv, hd, 16, seed=12)
+    blk = int(table[0, 1])
+    kv[blk, 0, 3, 1] = 255  # one K row of request 0, KV head 1
+    q = torch.randn(2, 4, hd, device="cuda", generator=_gen(4)).to(BF)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, splits=3)
+    assert got[0, 2:].isnan().all()
+    want, _ = _attn64(q, vals, 0.1)
+    assert got[0, :2].isfinite().all() and got[1].isfinite().all()
+    assert (got[1].double() - want[1]).abs().max() < 0.1
+
+
+def test_offsets_beyond_32_bits():
+    """Blocks more than 4 GiB into the pool, for each kernel that addresses it."""
+    hkv, hd, page = 2, 128, 16
+    row = kv4_ops.row_bytes(hd)
+    stride = 2 * page * hkv * row
+    far = 2 ** 32 // stride + 3
+    flat = torch.zeros((far + 2) * stride, dtype=torch.uint8, device="cuda")
+    kv = flat.view(far + 2, 2, page, hkv, row)
+    x = torch.randn(30, 3 * hkv, hd, device="cuda", generator=_gen(5)).to(BF)
+    slots = (torch.tensor([far, 1], device="cuda")[torch.arange(30, device="cuda") // 16] * page
+             + torch.arange(30, device="cuda") % 16)
+    q, k = torch.empty(30, hkv, hd, dtype=BF, device="cuda"), torch.empty(30, hkv, hd, dtype=BF, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(x, torch.arange(30, dtype=torch.int32, device="cuda"), _cos_sin(32, hd), hkv, hkv, kv,
+                                  slots, q_out=q, k_out=k)
+    kg, vg = kv4_ops.kv4_gather(kv, slots)
+    assert torch.equal(vg, kv4_ops.unpack_rows(kv4_ops.pack_rows(x[:, 2 * hkv:], True), True).to(BF))
+    vals = [(kv4_ops.unpack_rows(kv4_ops.pack_rows(k, False), False).double(),
+             kv4_ops.unpack_rows(kv4_ops.pack_rows(x[:, 2 * hkv:], True), True).double())]
+    got = kv4_ops.paged_decode_attn_kv4(q[29:], kv, _i32([[far, 1]]), _i32([30]), 0.1, splits=2)
+    _check_attn(got, q[29:], vals, 0.1)
+
+
+# ------------------------------------------------------- all of them together
+
+
+def _run_together(B=5, hq=8, hkv=2, hd=128, page=16):
+    """Two ragged steps of a batch: tables, write, decode attention over what was written."""
+    g = _gen(42)
+    pool = KvLayout.allocate(LayoutConfig.for_model(64, 2, hkv, kv4_ops.row_bytes(hd), page, torch.uint8),
+                             "fully_contiguous", KvBlockLayout.OPERATIONAL_NHD)
+    kv = pool.layer_view(1)
+    cs = _cos_sin(512, hd)
+    prompt = [33, 1, 16, 100, 47]
+    owned = [-(-(n + 1) // page) for n in prompt]
+    ids = _i32(torch.randperm(64, generator=torch.Generator().manual_seed(1))[: sum(owned)].tolist())
+    T = sum(prompt) + 6  # a padded batch
+    x = torch.randn(T, hq + 2 * hkv, hd, device="cuda", generator=g).to(BF)
+    y = torch.randn(B, hq + 2 * hkv, hd, device="cuda", generator=g).to(BF)
+    w = (1 + 0.1 * torch.randn(2, hd, device="cuda", generator=g)).to(BF)
+    return pool, kv, cs, prompt, owned, ids, T, x, y, w
+
+
+def _steps(kv, cs, prompt, owned, ids, T, x, y, w, hq=8, hkv=2, hd=128, page=16):
+    B = len(prompt)
+    t = table_ops.batch_tables(_i32(prompt), _i32([0] * B), ids, page=page, max_blocks=10, num_tokens=T,
+                               block_counts=_i32(owned))
+    q1 = torch.empty(T, hq, hd, dtype=BF, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(x, t.positions, cs, hq, hkv, kv, t.slots, q_weight=w[0], k_weight=w[1], q_out=q1)
+    pos = t.seq_lens  # the next token's position
+    slots = table_ops.slot_map(t.block_table, pos, page=page)
+    q2 = torch.empty(B, hq, hd, dtype=BF, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(y, pos, cs, hq, hkv, kv, slots, q_weight=w[0], k_weight=w[1], q_out=q2)
+    out = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, pos + 1, 1 / math.sqrt(hd), splits=2)
+    return t, q2, out
+
+
+def test_operators_together():
+    pool, kv, cs, prompt, owned, ids, T, x, y, w = _run_together()
+    t, q2, out = _steps(kv, cs, prompt, owned, ids, T, x, y, w)
+    page, vals, at, blk = 16, [], 0, 0
+    for b, n in enumerate(prompt):
+        mine = ids[blk: blk + owned[b]].long()
+        blk += owned[b]
+        assert t.block_table[b, : owned[b]].tolist() == mine.tolist()
+        p = torch.arange(n + 1, device="cuda")
+        k, v = kv4_ops.kv4_gather(kv, mine[p // page] * page + p % page)
+        raw = torch.cat([x[at: at + n], y[b: b + 1]])
+        assert torch.equal(v, kv4_ops.unpack_rows(kv4_ops.pack_rows(raw[:, 10:], True), True).to(BF))
+        (_, _), (k64, _) = _heads64(raw, p, cs, 8, 2, w[0], w[1], 1e-6)
+        span = k64.unflatten(-1, (-1, 32)).amax(-1) - k64.unflatten(-1, (-1, 32)).amin(-1)
+        err = (k.double() - k64).abs().unflatten(-1, (-1, 32)).amax(-1)
+        # half a step, the element's and the range's bf16 roundings, and the read-back's
+        assert (err <= span / 30 * (1 + 2.0 ** -7) + 3 * HALF_STEP * k64.unflatten(-1, (-1, 32)).abs().amax(-1)).all()
+        rows = kv[mine[p // page], :, p % page]
+        vals.append((kv4_ops.unpack_rows(rows[:, 0], False).double(), kv4_ops.unpack_rows(rows[:, 1], True).double()))
+        at += n
+    _check_attn(out, q2, vals, 1 / math.sqrt(128))
+
+
+def test_operators_together_captured_and_on_another_stream():
+    pool, kv, cs, prompt, owned, ids, T, x, y, w = _run_together()
+    _, _, want = _steps(kv, cs, prompt, owned, ids, T, x, y, w)
+    want = want.clone()
+    args = (_i32(prompt), _i32([0] * 5), ids, _i32(owned))
+
+    def step(stream=None):
+        t = table_ops.batch_tables(args[0], args[1], args[2], page=16, max_blocks=10, num_tokens=T,
+                                   block_counts=args[3], stream=stream)
+        q1 = torch.empty(T, 8, 128, dtype=BF, device="cuda")
+        kv4_ops.qk_norm_rope_kv_write(x, t.positions, cs, 8, 2, kv, t.slots, q_weight=w[0], k_weight=w[1], q_out=q1,
+                                      stream=stream)
+        slots = table_ops.slot_map(t.block_table, t.seq_lens, page=16, stream=stream)
+        q2 = torch.empty(5, 8, 128, dtype=BF, device="cuda")
+        kv4_ops.qk_norm_rope_kv_write(y, t.seq_lens, cs, 8, 2, kv, slots, q_weight=w[0], k_weight=w[1], q_out=q2,
+                                      stream=stream)
+        return t, q1, q2, slots
+
+    kv.zero_()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    t, q1, q2, slots = step(stream=s)
+    got = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, _i32([n + 1 for n in prompt]), 1 / math.sqrt(128),
+                                        splits=2, stream=s.cuda_stream)
+    s.synchronize()
+    assert torch.equal(got, want)
+    kv.zero_()
+    graph = torch.cuda.CUDAGraph()
+    seq = _i32([n + 1 for n in prompt])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        t, q1, q2, slots = step()
+        got = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, seq, 1 / math.sqrt(128), splits=2)
+    for _ in range(2):
+        kv.zero_()
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

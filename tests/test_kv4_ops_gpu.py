@@ -277,27 +277,38 @@ def _filled(B, lens, heads, hd, page, order="nhd", seed=0, spread=1.0):
             n = min(page, lens[b] - j * page)
             kv[int(table[b, j]), 0, :n] = rk[j * page: j * page + n]
             kv[int(table[b, j]), 1, :n] = rv[j * page: j * page + n]
-        vals.append((kv4_ops.unpack_rows(rk[: lens[b]], False).double(), kv4_ops.unpack_rows(rv[: lens[b]], True).double()))
+        vals.append(_values(rk[: lens[b]], rv[: lens[b]]))
     return kv, table, vals
 
 
 def _attn64(q, vals, scale):
+    """The result in 64 bits, and sum p |v - v8|: v8 = zero + 8 scale is the value of a group's code 8."""
     B, hq, hd = q.shape
     out, size = torch.zeros(2, B, hq, hd, dtype=torch.float64, device="cuda")
-    for b, (k, v) in enumerate(vals):
+    for b, (k, v, v8) in enumerate(vals):
         if k.shape[0]:
             rep = hq // k.shape[1]
-            kk, vv = k.repeat_interleave(rep, 1), v.repeat_interleave(rep, 1)
+            kk, vv, mm = (x.repeat_interleave(rep, 1) for x in (k, v, v8))
             p = torch.softmax(torch.einsum("hd,nhd->hn", q[b].double(), kk) * scale, -1)
             out[b] = torch.einsum("hn,nhd->hd", p, vv)
-            size[b] = torch.einsum("hn,nhd->hd", p, vv.abs())
+            size[b] = torch.einsum("hn,nhd->hd", p, vv.abs() + (vv - mm).abs())
     return out, size
+
+
+def _values(rk, rv):
+    """(k, v, v8) in 64 bits of 4-bit rows."""
+    hd = {48: 64, 80: 128, 160: 256}[rv.shape[-1]]
+    par = rv[..., hd // 2: hd // 2 + hd // 8].contiguous().view(BF).double().unflatten(-1, (-1, 2))
+    v8 = (par[..., 1] + 8 * par[..., 0]).repeat_interleave(32, -1)
+    return kv4_ops.unpack_rows(rk, False).double(), kv4_ops.unpack_rows(rv, True).double(), v8
 
 
 def _check_attn(got, q, vals, scale, **kw):
     want, size = _attn64(q, vals, scale)
-    # one rounding of the result to bf16 and one of each weight p (relative 2^-8 each, so of sum p |v|); scores
-    # carry fp32 rounding of |scale q . k| terms, far below: another 2^-10 of sum p |v|
+    # One rounding of the result to bf16: half a step of it. The kernel sums p (zero + 8 scale) in fp32 and
+    # bf16(p scale) (code - 8) on tensor cores: the rounding is off by at most half a step of p scale, and scale
+    # |code - 8| is |v - v8|, so of sum p |v - v8|. Scores carry fp32 rounding, far below: 2^-10 of sum p |v|.
+    # (`size` holds both sums, so each bound is taken of a little more than its own.)
     bound = HALF_STEP * want.abs() + (HALF_STEP + 2.0 ** -10) * size + 1e-30
     err = (got.double() - want).abs()
     assert (err <= bound).all(), (float((err - bound).max()), float(err.max()))
@@ -348,7 +359,7 @@ def test_attention_strided_query_table_and_caller_buffers():
     # a table wider than the sequences need, and lengths beyond the table's width
     _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, big, _i32(lens), 0.1), q, vals, 0.1)
     full = table[:, :1].contiguous()
-    vals1 = [(k[:16], v[:16]) for k, v in vals]
+    vals1 = [tuple(x[:16] for x in v) for v in vals]
     _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, full, _i32([90, 2 ** 31 - 1, 17]), 0.1), q, vals1, 0.1)
     none = kv4_ops.paged_decode_attn_kv4(q, kv, table[:, :0], _i32(lens), 0.1)
     assert not none.any()
@@ -363,7 +374,7 @@ def test_attention_pages_outside_the_pool_hold_no_tokens():
             torch.zeros(64, dtype=torch.bool, device="cuda")]
     q = torch.randn(3, 8, hd, device="cuda", generator=_gen(2)).to(BF)
     got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.2, splits=2)
-    _check_attn(got, q, [(k[m], v[m]) for (k, v), m in zip(vals, keep)], 0.2)
+    _check_attn(got, q, [tuple(x[m] for x in v) for v, m in zip(vals, keep)], 0.2)
     assert not got[2].any()
 
 
@@ -391,7 +402,7 @@ def test_attention_one_token_far_above_many():
         kv[int(table[0, j]), 0], kv[int(table[0, j]), 1] = rk[16 * j: 16 * j + 16], rv[16 * j: 16 * j + 16]
     q = torch.zeros(1, 1, hd, device="cuda", dtype=BF)
     q[0, 0, 0] = 1.0
-    vals = [(kv4_ops.unpack_rows(rk, False).double(), kv4_ops.unpack_rows(rv, True).double())]
+    vals = [_values(rk, rv)]
     for splits in (1, 8):
         got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, splits=splits)
         _check_attn(got, q, vals, 1.0)
@@ -426,8 +437,7 @@ def test_offsets_beyond_32_bits():
                                   slots, q_out=q, k_out=k)
     kg, vg = kv4_ops.kv4_gather(kv, slots)
     assert torch.equal(vg, kv4_ops.unpack_rows(kv4_ops.pack_rows(x[:, 2 * hkv:], True), True).to(BF))
-    vals = [(kv4_ops.unpack_rows(kv4_ops.pack_rows(k, False), False).double(),
-             kv4_ops.unpack_rows(kv4_ops.pack_rows(x[:, 2 * hkv:], True), True).double())]
+    vals = [_values(kv4_ops.pack_rows(k, False), kv4_ops.pack_rows(x[:, 2 * hkv:], True))]
     got = kv4_ops.paged_decode_attn_kv4(q[29:], kv, _i32([[far, 1]]), _i32([30]), 0.1, splits=2)
     _check_attn(got, q[29:], vals, 0.1)
 
@@ -484,7 +494,7 @@ def test_operators_together():
         # half a step, the element's and the range's bf16 roundings, and the read-back's
         assert (err <= span / 30 * (1 + 2.0 ** -7) + 3 * HALF_STEP * k64.unflatten(-1, (-1, 32)).abs().amax(-1)).all()
         rows = kv[mine[p // page], :, p % page]
-        vals.append((kv4_ops.unpack_rows(rows[:, 0], False).double(), kv4_ops.unpack_rows(rows[:, 1], True).double()))
+        vals.append(_values(rows[:, 0], rows[:, 1]))
         at += n
     _check_attn(out, q2, vals, 1 / math.sqrt(128))
 

@@ -276,7 +276,7 @@ def run(state):
         if op == "read":
             return list(kv4_ops.kv4_gather(state["kv"], state["slots"]))
         return [kv4_ops.paged_decode_attn_kv4(state["q"], state["kv"], state["block_table"], state["seq_lens"],
-                                              state["scale"], counters=state["counters"])]
+                                              state["scale"])]
     if op == "tables":
         return _plain_tables(state)
     if op == "slots":

@@ -251,36 +251,66 @@ extern "C" int kvbm_kv4_gather(const void* kv, int64_t block_stride, int64_t out
   return cudaGetLastError();
 }
 
-// Scratch: part_acc batch * hq * splits * hd floats, part_ml twice batch * hq * splits.
-// `counters` (batch * hkv * ceil(hq / hkv / 8) zeros, left zero again) merges the
-// splits in the last CTA of each (request, head group); null: a second launch does.
+// How a launch of the decode attention is laid out: out[0] floats of scratch, out[1]
+// CTAs along the work. `ctas` 0: one for each the GPU holds at a time.
+extern "C" int kvbm_paged_decode_attn_kv4_plan(int batch, int hq, int hkv, int hd, int64_t max_tokens, int ctas,
+                                               int sm_count, int64_t* out) {
+  if (!out || batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || max_tokens < 0 || ctas < 0 || sm_count <= 0)
+    return cudaErrorInvalidValue;
+  const kv4::Plan p = kv4::plan_decode(batch, hq, hkv, hd, max_tokens, ctas, sm_count);
+  out[0] = static_cast<int64_t>(p.ctas) * 2 * hq * (hd + 2) + 2 * (static_cast<int64_t>(batch) + 1);
+  out[1] = p.ctas;
+  return cudaSuccess;
+}
+
+// `scratch`: 16-byte aligned floats as the plan says.
 extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const void* kv, int64_t block_stride,
                                           int64_t outer_stride, int64_t token_stride, int64_t head_stride, int page,
                                           int num_blocks, const int32_t* block_table, int64_t table_stride,
                                           int max_blocks, const int32_t* seq_lens, int batch, int hq, int hkv, int hd,
-                                          float softmax_scale, int splits, float* part_acc, float* part_ml,
-                                          unsigned int* counters, void* out, cudaStream_t stream) {
+                                          float softmax_scale, int ctas, int sm_count, float* scratch, void* out,
+                                          cudaStream_t stream) {
   if (batch == 0) return cudaSuccess;
   kv4::AttnParams P{};
   P.cache = Cache{static_cast<uint8_t*>(const_cast<void*>(kv)), block_stride, outer_stride, token_stride, head_stride,
                   page, num_blocks, hkv};
   if (batch < 0 || batch > 65535 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || !cache_ok(P.cache) || !q || !aligned16(q) ||
       q_stride % 8 != 0 || !out || !aligned16(out) || !seq_lens || max_blocks < 0 || (max_blocks > 0 && !block_table) ||
-      splits <= 0 || (splits > 1 && (!part_acc || !part_ml)))
+      ctas < 0 || sm_count <= 0 || !scratch || !aligned16(scratch))
     return cudaErrorInvalidValue;
+  const kv4::Plan plan =
+      kv4::plan_decode(batch, hq, hkv, hd, static_cast<int64_t>(max_blocks) * page, ctas, sm_count);
+  if (plan.y_ctas > 65535 || static_cast<int64_t>(batch) * hq > 0x7fffffff) return cudaErrorInvalidValue;
   P.q = static_cast<const __nv_bfloat16*>(q);
   P.q_stride = q_stride;
   P.table = block_table;
   P.table_stride = table_stride;
   P.max_blocks = max_blocks;
   P.seq_lens = seq_lens;
+  P.batch = batch;
   P.hq = hq;
   P.group = hq / hkv;
+  P.chunks = plan.chunks;
+  P.y_total = plan.y_total;
+  P.y_cta = plan.y_cta;
+  P.streams = plan.streams;
   P.qscale = softmax_scale * 1.4426950408889634f;  // log2(e)
-  P.part_acc = part_acc;
-  P.part_ml = part_ml;
-  P.counters = counters;
+  const int64_t rows = static_cast<int64_t>(plan.ctas) * 2 * hq;
+  P.part_acc = scratch;
+  P.part_ml = scratch + rows * hd;
+  P.first = reinterpret_cast<int64_t*>(scratch + rows * (hd + 2));
   P.out = static_cast<__nv_bfloat16*>(out);
   P.page_div = FastDiv(static_cast<uint32_t>(page));
-  return kv4::launch_decode(P, batch, hd, splits, stream);
+  return kv4::launch_decode(P, hd, plan, stream);
+}
+
+// 0, or the status a launch recorded (3 = a wait for a copy gave up); synchronizes.
+extern "C" int kvbm_kv4_status(int reset) {
+  int v = -1;
+  if (cudaMemcpyFromSymbol(&v, kv4::g_kv4_status, sizeof(int)) != cudaSuccess) return -1;
+  if (reset) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(kv4::g_kv4_status, &zero, sizeof(int));
+  }
+  return v;
 }

@@ -227,13 +227,17 @@ int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t tokens, in
 int kvbm_kv4_gather(const void* kv, int64_t block_stride, int64_t outer_stride, int64_t token_stride,
                     int64_t head_stride, int page, int num_blocks, int heads, int hd, const int64_t* slots,
                     int64_t tokens, void* k_out, void* v_out, cudaStream_t stream);
-// Decode attention over the 4-bit cache; q and out [batch, hq, hd] bf16.
+// Decode attention over the 4-bit cache; q and out [batch, hq, hd] bf16. The plan says how many floats of
+// scratch a launch takes.
+int kvbm_paged_decode_attn_kv4_plan(int batch, int hq, int hkv, int hd, int64_t max_tokens, int ctas, int sm_count,
+                                    int64_t* out);
 int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const void* kv, int64_t block_stride,
                                int64_t outer_stride, int64_t token_stride, int64_t head_stride, int page,
                                int num_blocks, const int32_t* block_table, int64_t table_stride, int max_blocks,
                                const int32_t* seq_lens, int batch, int hq, int hkv, int hd, float softmax_scale,
-                               int splits, float* part_acc, float* part_ml, unsigned int* counters, void* out,
-                               cudaStream_t stream);
+                               int ctas, int sm_count, float* scratch, void* out, cudaStream_t stream);
+// 0, or 3 when a launch of the attention gave a copy up (its result is NaN); synchronizes.
+int kvbm_kv4_status(int reset);
 
 #ifdef __cplusplus
 }

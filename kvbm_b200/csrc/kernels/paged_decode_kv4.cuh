@@ -2,45 +2,62 @@
 //
 //   out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = 2^(s_t - m),  s_t = qscale q . k_t,  t < seq_lens[b]
 //
-// in one pass with a running maximum m and sum. The sequence is cut into
-// `splits` ranges; a CTA takes one range of one (request, KV head, up to 8 query
-// heads), its 4 warps every 4th tile of 32 tokens, and the (m, l, acc) of warps
-// and ranges are merged at the end.
+// in one pass with a running maximum m and sum.
 //
 // What bounds it: at the HBM rate an SM gets the 160 bytes of a (token, KV head)
-// of 128 elements every 7 cycles, so about 28 warp instructions are all there is
-// for unpacking 256 codes, both products and the softmax. Hence warp-level
-// mma.sync with the codes turned into operands in registers, rather than
-// tcgen05, whose operands would have to be written back to shared memory first
-// (and whose block scales run along the contraction, which for P V is the
-// tokens: the wrong way). The arithmetic is arranged so that no element is
+// of 128 elements every 7 cycles, in which it issues 28 warp instructions, 14 of
+// them on the integer pipe. That is all there is for unpacking 256 codes, both
+// products and the softmax. Hence warp-level mma.sync with the codes turned into
+// operands in registers, rather than tcgen05, whose operands would have to be
+// written back to shared memory first (and whose block scales run along the
+// contraction, which for P V is the tokens: the wrong way). No element is
 // dequantised:
 //
-// Scores. A nibble c read as an e4m3 byte is c 2^-9, exactly (0..7 are its
-// subnormals, 8..15 its first binade). q is split into two e4m3 parts
-// q 2^k = hi + lo, which together hold a bf16's 8 bits (exact for elements down
-// to 2^-9 of the head's largest; below, off by at most 2^-18 of it). One
-// m16n8k32 product covers one group of 32, and its scale and zero are applied to
-// the fp32 sums:  q . k = sum_g s_g (c . q_g) + z_g (sum of q_g).
+// A nibble masked in place is a subnormal fp16: c 2^-24 in bits 0-3, c 2^-20 in
+// bits 4-7, both exact. So a word of 8 codes becomes 4 operand registers with
+// one shift and four ands, and the factor 16 goes to the other operand (scores)
+// or to the end (P V).
 //
-// P V. A nibble c or'ed into 0x4300 is the bf16 128 + c. Codes of two tokens are
-// paired by one byte permute, the V scale goes into the weight, p' = bf16(p s):
+// Scores. q 2^k in fp16 is exact (bf16 has 8 bits; k puts the head's largest
+// element at 2^14, elements below 2^-28 of it lose bits). Each group of 32 is two
+// m16n8k16 products, whose fp32 sums take the group's scale; the zeros' part,
+// sum over g of z_g (sum of q_g), is one bf16 product more with the sums of q in
+// three bf16 parts.
 //
-//   acc = sum p' (128 + c),  W = sum p' (a product with ones),  Z = sum p (z + 8 s)
-//   sum p v = acc - 136 W + Z
+// P V. Codes of two tokens are paired by one byte permute. The V scale goes into
+// the weight: p' = fp16(p s f), off by at most 2^-11 of it, with f a power of
+// two that keeps the warp's largest s f in [2^13, 2^15]; f changes, and the sums
+// with it, when a larger scale comes by. Then sum p v = sum p' c / f + sum p z.
+// Products of 32 tokens are folded into fp32 accumulators, since the tensor
+// core's own accumulation truncates.
 //
-// so p' only multiplies c - 8, never the offset. Products of 32 tokens are folded
-// into fp32 accumulators, since the tensor core's own accumulation truncates.
+// With up to 4 query heads on a KV head (PAIR) the 8 columns of a P V product
+// hold p' of 4 heads for two groups: tile rows 0-7 are elements of the even
+// group, rows 8-15 of the odd one, half of the outputs have no meaning. With 5
+// to 8 heads a column is a head and a tile lies in one group.
 //
-// With up to 4 query heads (PAIR) the 8 columns of a product hold hi and lo of
-// 4 heads for the scores, and for P V the p' of 4 heads for two groups: tile
-// rows 0-7 are elements of the even group, rows 8-15 of the odd one, half of the
-// outputs have no meaning. With 5 to 8 heads hi and lo are two products and a
-// tile lies in one group.
+// Work. A warp takes one (KV head, up to 8 query heads) and tiles of 32 tokens;
+// the warps of a CTA take different KV heads of the same tokens (with fewer than
+// 8, several streams of tokens), so that what lies together in a token-first pool
+// is read together. All requests' tiles are laid end to end and cut into equal
+// ranges, one for each CTA the GPU holds at a time, so ragged batches and odd
+// numbers of heads cost no idle SMs. A CTA meets at most two requests that are
+// not its own alone; their partial results (m, l, acc) are merged by a second
+// kernel, whose launch overlaps the first's end.
+//
+// Copies. Each warp has its own ring of two tiles. A unit of 16 tokens, K and V
+// rows of one KV head, is one TMA box of the five-dimensional pool, issued by the
+// lane that looked the unit's page up (32 units at a time); where a page is not a
+// multiple of 16 tokens, rows are copied one by one with cp.async.
 #pragma once
 
 #include "common.cuh"
 #include "kv4_format.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
 
 namespace kvbm {
 namespace kv4 {
@@ -53,40 +70,25 @@ struct AttnParams {
   int64_t table_stride;
   int max_blocks;
   const int32_t* seq_lens;
-  int hq, group;
+  int batch, hq, group, chunks;  // chunks: groups of up to 8 query heads on a KV head
+  int y_total, y_cta, streams;   // (KV head, chunk) pairs: in all, a CTA; streams of tokens a CTA
   float qscale;
-  float* part_acc;
-  float* part_ml;
-  unsigned int* counters;
+  float* part_acc;  // [cta][2][hq][HD]
+  float* part_ml;   // [cta][2][hq][2]
+  int64_t* first;   // [batch] first round of a request, then the rounds a CTA takes; for the merge kernel
   __nv_bfloat16* out;
   FastDiv page_div;
 };
 
-constexpr int kHeads = 8;  // query heads a CTA takes at most
-constexpr int kAttnWarps = 4;
-constexpr int kUnit = 16;  // tokens a stage of the ring holds
-constexpr int kTile = 32;  // tokens a warp takes between two updates of its accumulators
+constexpr int kHeads = 8;       // query heads a warp takes at most
+constexpr int kMaxWarps = 8;
+constexpr int kUnit = 16;       // tokens a stage of the ring holds
+constexpr int kTile = 32;       // tokens a warp takes between two updates of its accumulators
+constexpr int kStages = 4;      // two tiles of two units
+constexpr int kMinRounds = 2;   // a CTA takes at least so many tiles a warp: below, merging costs more than it saves
+constexpr uint64_t kWaitNs = 1000000000ull;  // after which a warp gives a copy up
 
-// Merges the splits of one query head's row: thread d of HD.
-template <int HD>
-__device__ __forceinline__ void merge_row(const AttnParams& P, int64_t bh, int splits, int d) {
-  float M = -INFINITY;
-  for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(&P.part_ml[(bh * splits + s) * 2]));
-  float l = 0.f, a = 0.f;
-  for (int s = 0; s < splits; ++s) {
-    const float ls = __ldcg(&P.part_ml[(bh * splits + s) * 2 + 1]);
-    if (ls == 0.f) continue;  // no tokens (a NaN goes on)
-    const float f = exp2f(__ldcg(&P.part_ml[(bh * splits + s) * 2]) - M);
-    l += f * ls;
-    a += f * __ldcg(&P.part_acc[(bh * splits + s) * HD + d]);
-  }
-  P.out[bh * HD + d] = __float2bfloat16(l == 0.f ? 0.f : a / l);
-}
-
-template <int HD>
-__global__ void __launch_bounds__(HD) kv4_merge_kernel(const __grid_constant__ AttnParams P, int splits) {
-  merge_row<HD>(P, blockIdx.x, splits, threadIdx.x);
-}
+__device__ int g_kv4_status = 0;
 
 // ---- instructions ----------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) {
@@ -94,23 +96,22 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
+// d = a b + c; the first product of a chain takes zeros for c, which costs no registers.
+#define KVBM_KV4_MMA(NAME, TYPE)                                                                                     \
+  __device__ __forceinline__ void NAME(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,            \
+                                       uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {           \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                                       \
+        ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"                                             \
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                             \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));                 \
+  }
+KVBM_KV4_MMA(mma_f16, "f16")
+KVBM_KV4_MMA(mma_bf16, "bf16")
+#undef KVBM_KV4_MMA
 // Transposes the 8x8 matrix of 16-bit elements whose row lane / 4 this lane holds in columns 2 (lane % 4) + {0, 1}.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ void copy16(uint32_t smem, const void* gmem) {
@@ -134,469 +135,739 @@ __device__ __forceinline__ void lds(uint32_t (&x)[WORDS], uint32_t addr) {
                    : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3])
                    : "r"(addr + 4 * i));
 }
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
+// K and V rows of `kUnit` tokens of one KV head: coordinates (byte, head, token in the page, K / V, block).
+__device__ __forceinline__ void copy_unit(uint32_t smem, const CUtensorMap* map, int head, int token, int block,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(smem),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(token), "r"(0), "r"(block), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ float e4m3_part(float x, bool low) {
-  __nv_fp8_e4m3 h(x);
-  return low ? x - static_cast<float>(h) : x;
+__device__ __forceinline__ uint32_t half2(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
 }
-// Code i of two tokens' packed codes y (one token a half word) as the bf16 pair 128 + c.
-__device__ __forceinline__ uint32_t code_pair(uint32_t y, int i) { return ((y >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
+// Nibbles i and i + 4 of x as an fp16 pair, times 2^-24 (i even) or 2^-20 (i odd).
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, int i) {
+  return (i < 2 ? x : x >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+__device__ __forceinline__ int exponent(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127; }
+
+__device__ __forceinline__ int tokens_of(const AttnParams& P, int b) {
+  return static_cast<int>(min(static_cast<int64_t>(max(P.seq_lens[b], 0)),
+                              min(static_cast<int64_t>(P.max_blocks) * P.cache.page, static_cast<int64_t>(0x7ffff000))));
+}
+// Rounds of streams x 32 tokens; an empty request has one, so that its zeros are written like any result.
+__device__ __forceinline__ int rounds_of(int tokens, int streams) {
+  return max((tokens + kTile * streams - 1) / (kTile * streams), 1);
+}
+// Merges the partial results of each request that several CTAs worked on. Part i of a request that begins in
+// CTA c lies in CTA c + i, in the slot of that CTA's first request (0), or of a later one (1: only its last can go
+// on). A warp reads 32 parts' (m, l), a lane each, and up to 16 parts' acc at a time, lane l elements l E ..
+// (E = HD / 32). A CTA takes `heads_cta` query heads of a request: few parts are merged by one warp a head, many by
+// all warps, head by head.
+constexpr int kMergeWarps = 8;
+template <int HD>
+__device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, int64_t slot0, int begin, int step, int n,
+                                            float& m, float& l, float (&acc)[HD / 32]) {
+  constexpr int E = HD / 32, V = E < 4 ? E : 4, kFly = 64 / E;
+  const int lane = threadIdx.x & 31;
+  auto row = [&](int i) { return row0 + static_cast<int64_t>(i) * 2 * P.hq + (i == 0 ? slot0 : 0); };
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int i0 = begin; i0 < n; i0 += step) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (i0 + lane < n) ml = __ldcg(reinterpret_cast<const float2*>(P.part_ml) + row(i0 + lane));
+    const float top = fmaxf(m, warp_max(ml.x));
+    const float down = l == 0.f ? 0.f : exp2f(m - top);
+    const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - top);  // no tokens: nothing (a NaN goes on)
+    l = fmaf(l, down, warp_sum(f * ml.y));
+    m = top;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= down;
+    const int here = min(32, n - i0);
+    for (int j = 0; j < here; j += kFly) {
+      float x[kFly][E];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        if (j + k >= here) break;
+        const float* src = P.part_acc + row(i0 + j + k) * HD + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += V) {
+          if constexpr (V == 2)
+            *reinterpret_cast<float2*>(&x[k][e]) = __ldcg(reinterpret_cast<const float2*>(src + e));
+          else
+            *reinterpret_cast<float4*>(&x[k][e]) = __ldcg(reinterpret_cast<const float4*>(src + e));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        if (j + k >= here) break;
+        const float fk = __shfl_sync(0xffffffffu, f, j + k);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(fk, x[k][e], acc[e]);
+      }
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __grid_constant__ AttnParams P,
+                                                                     int heads_cta) {
+  constexpr int E = HD / 32;
+  __shared__ float red[kMergeWarps][HD + 2];
+  const int b = blockIdx.y, h_begin = blockIdx.x * heads_cta, h_end = min(P.hq, h_begin + heads_cta);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rounds = rounds_of(tokens_of(P, b), P.streams);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t first = P.first[b], per = P.first[P.batch];
+  const int64_t c0 = first / per;
+  const int n = static_cast<int>((first + rounds - 1) / per - c0) + 1;
+  if (n == 1) return;  // written by its one CTA
+  const int64_t slot0 = first == c0 * per ? 0 : P.hq;
+  const bool few = n <= 32;
+  for (int h = h_begin + (few ? warp : 0); h < h_end; h += few ? kMergeWarps : 1) {
+    float m, l, acc[E];
+    merge_parts<HD>(P, c0 * 2 * P.hq + h, slot0, few ? 0 : warp * 32, kMergeWarps * 32, n, m, l, acc);
+    if (!few) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) red[warp][lane * E + e] = acc[e];
+      if (lane == 0) {
+        red[warp][HD] = m;
+        red[warp][HD + 1] = l;
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+      m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, red[w][HD]);
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) {
+        const float lw = red[w][HD + 1];
+        const float f = lw == 0.f ? 0.f : exp2f(red[w][HD] - m);
+        l = fmaf(f, lw, l);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, red[w][lane * E + e], acc[e]);
+      }
+    }
+    const float r = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(P.out + (static_cast<int64_t>(b) * P.hq + h) * HD + lane * E);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = pack2(acc[e] * r, acc[e + 1] * r);
+  }
+}
 
 template <int HD>
 struct Geometry {
   static constexpr int NG = HD / kGroup;
   static constexpr int kRow = row_bytes(HD);
-  static constexpr int kChunks = kRow / 16;                  // 16-byte pieces a row; also copies a lane per unit
-  static constexpr int kSmemRow = kRow + (HD == 256 ? 16 : 0);  // rows 8 apart in banks of 4 words: no conflicts
-  static constexpr int kUnitBytes = 2 * kUnit * kSmemRow;    // K rows, then V rows
-  static constexpr int kStages = 4;
-  static constexpr int kCtasPerSm = HD == 256 ? 2 : 4;
-  static constexpr int kSmem = kAttnWarps * kStages * kUnitBytes;
+  static constexpr int kChunks = kRow / 16;        // 16-byte pieces a row; also copies a lane for a unit
+  static constexpr int kUnitBytes = 2 * kUnit * kRow;  // K rows, then V rows
+  static constexpr int kCtasPerSm = HD == 256 ? 1 : 2;  // of 8 warps
+  static constexpr int kRingBytes = kStages * kUnitBytes;  // a warp
 };
 
-template <int HD, bool PAIR, bool SMALL_PAGE>
-__global__ void __launch_bounds__(kAttnWarps * 32, Geometry<HD>::kCtasPerSm)
-    kv4_decode_kernel(const __grid_constant__ AttnParams P) {
+template <int HD, bool PAIR, bool TMA>
+__global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
+    kv4_decode_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map) {
   using G = Geometry<HD>;
   constexpr int NG = G::NG;
-  constexpr int NH = PAIR ? 1 : 2;             // query heads whose scores a lane holds
-  constexpr int NW = NG / 2;                   // words of V codes a lane takes from a row
+  constexpr int NH = PAIR ? 1 : 2;       // query heads whose scores a lane holds
+  constexpr int NW = NG / 2;             // words of V codes a lane takes from a row
+  constexpr int NZ = (NG + 3) / 4;       // products for the zeros of K
+  constexpr int NB = PAIR ? NG / 2 : NG; // operands of weights a unit
   extern __shared__ __align__(128) uint8_t smem[];
-  const int splits = gridDim.x, split = blockIdx.x, b = blockIdx.z;
-  const int chunks = (P.group + kHeads - 1) / kHeads;
-  const int kvh = blockIdx.y / chunks, h0 = (blockIdx.y - kvh * chunks) * kHeads;
-  const int heads = min(kHeads, P.group - h0);
-  const int64_t bh0 = static_cast<int64_t>(b) * P.hq + kvh * P.group + h0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;");  // the merge may be put in place; it waits for this grid's end
+  __shared__ uint64_t full[kMaxWarps][2];  // a warp's two tiles
+  if constexpr (TMA) {
+    if (lane < 2) mbar_init(&full[warp][lane], 2);  // the two lanes that issue its units
+    fence_mbar_init();
+    if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
+  }
 
-  const int64_t seq = min(static_cast<int64_t>(max(P.seq_lens[b], 0)),
-                          static_cast<int64_t>(P.max_blocks) * P.cache.page);
-  // ranges of whole rounds of the 4 warps, so that no warp of a long range idles
-  constexpr int kRound = kAttnWarps * kTile;
-  const int64_t per = ((seq + splits - 1) / splits + kRound - 1) / kRound * kRound;
-  const int64_t t_begin = min(seq, split * per);
-  const int count = static_cast<int>(min(seq, t_begin + per) - t_begin);  // tokens of this range
-  const int tiles = (count + kTile - 1) / kTile;
-  const int mine = tiles > warp ? (tiles - warp + kAttnWarps - 1) / kAttnWarps : 0;
-
-  // ---- q as e4m3 operands: column gid is head gid / 2, part gid % 2 (PAIR) or head gid
-  uint32_t bq[PAIR ? 1 : 2][NG][2];
-  float factor[NH], qsum[NH][NG];
+  // ---- this CTA's range of rounds, and the request it begins in
+  __shared__ int64_t warp_sum[kMaxWarps];
+  __shared__ int64_t start_first;
+  __shared__ int start_b;
+  int64_t f, f_end, per;
   {
-    const int h = PAIR ? gid >> 1 : gid;
-    float x[NG][8];
-    float top = 0.f;
-    bool bad = false;
+    const int each = (P.batch + blockDim.x - 1) / blockDim.x;
+    const int b0 = min(P.batch, static_cast<int>(threadIdx.x) * each), b1 = min(P.batch, b0 + each);
+    int64_t sum = 0;
+    for (int b = b0; b < b1; ++b) sum += rounds_of(tokens_of(P, b), P.streams);
+    int64_t run = sum;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      int4 w = make_int4(0, 0, 0, 0);
-      if (h < heads)
-        w = *reinterpret_cast<const int4*>(P.q + b * P.q_stride + (kvh * P.group + h0 + h) * static_cast<int64_t>(HD) +
-                                           g * kGroup + tig * 8);
-      const uint32_t ww[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[g][2 * k] = bf_lo(ww[k]);
-        x[g][2 * k + 1] = bf_hi(ww[k]);
-        top = fmaxf(top, fmaxf(fabsf(x[g][2 * k]), fabsf(x[g][2 * k + 1])));
-        bad |= (ww[k] & 0x7f80u) == 0x7f80u || (ww[k] & 0x7f800000u) == 0x7f800000u;
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += x;
     }
-    int flag = bad;
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      flag |= __shfl_xor_sync(0xffffffffu, flag, o);
+    if (lane == 31) warp_sum[warp] = run;
+    __syncthreads();
+    int64_t before = run - sum, total = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
+      if (w < warp) before += warp_sum[w];
+      total += warp_sum[w];
     }
-    // a power of two that brings the largest element to [128, 256)
-    const int e = max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100);
-    const float up = flag ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + 7 - e) << 23);
-    const float f = flag ? __uint_as_float(0x7fc00000u) : ldexpf(P.qscale, 9 + e - 7);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[g][k] = flag ? 0.f : x[g][k] * up;
-        s += x[g][k];
+    per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinRounds));
+    f = blockIdx.x * per;
+    f_end = min(total, f + per);
+    if (f >= total) return;
+    if (before <= f && f < before + sum) {
+      int b = b0;
+      for (; b < b1 - 1; ++b) {
+        const int n = rounds_of(tokens_of(P, b), P.streams);
+        if (f < before + n) break;
+        before += n;
       }
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-#pragma unroll
-      for (int n = 0; n < NH; ++n)
-        qsum[n][g] = 0.001953125f * __shfl_sync(0xffffffffu, s, 8 * tig + 4 * n);  // 2^-9, the codes' unit
-#pragma unroll
-      for (int part = 0; part < (PAIR ? 1 : 2); ++part) {
-        const bool low = PAIR ? (gid & 1) != 0 : part == 1;
-#pragma unroll
-        for (int odd = 0; odd < 2; ++odd)  // even elements meet the low nibbles, odd ones the high
-          bq[part][g][odd] = e4m3x4(e4m3_part(x[g][odd], low), e4m3_part(x[g][2 + odd], low),
-                                    e4m3_part(x[g][4 + odd], low), e4m3_part(x[g][6 + odd], low));
-      }
+      start_b = b;
+      start_first = before;
     }
-#pragma unroll
-    for (int n = 0; n < NH; ++n) factor[n] = __shfl_sync(0xffffffffu, f, 8 * tig + 4 * n);
+    __syncthreads();
   }
+  const int64_t f_begin = f;
+  int b = start_b;
+  int64_t first = start_first;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) P.first[P.batch] = per;
 
-  // ---- the ring: every lane copies kChunks pieces of a unit
-  const uint32_t ring = smem_u32(smem) + warp * (G::kStages * G::kUnitBytes);
-  int64_t from[G::kChunks];
-  uint32_t to[G::kChunks];
-#pragma unroll
-  for (int i = 0; i < G::kChunks; ++i) {
-    const int c = lane + 32 * i, v = c >= kUnit * G::kChunks;
-    const int r = c / G::kChunks - (v ? kUnit : 0), piece = c % G::kChunks;
-    from[i] = (v ? P.cache.outer_stride : 0) + (SMALL_PAGE ? 0 : r * P.cache.token_stride) + piece * 16;
-    to[i] = (v * kUnit + r) * G::kSmemRow + piece * 16;
-  }
-  const int32_t* table = P.table + b * P.table_stride;
-  const uint8_t* base = P.cache.base + static_cast<int64_t>(kvh) * P.cache.head_stride;
-  // block ids of the next 32 units, one a lane (-1: no tokens there)
-  int32_t ids = -1;
-  auto fetch_ids = [&](int tile) {  // for local tiles [tile, tile + 16)
-    const int64_t t = static_cast<int64_t>(warp + (tile + (lane >> 1)) * kAttnWarps) * kTile + (lane & 1) * kUnit;
-    ids = -1;
-    if (t < count) {
-      ids = table[P.page_div.div(static_cast<uint32_t>(t_begin + t))];
-      if (static_cast<uint32_t>(ids) >= static_cast<uint32_t>(P.cache.num_blocks)) ids = -1;
-    }
-  };
-  // tokens of unit 0 / 1 of the tile in flight that count, a bit each (16 of each)
-  uint32_t live_next = 0u;
-  auto issue = [&](int tile) {
-    uint32_t live = 0u;
-    if (tile < mine) {
-      if (!SMALL_PAGE && (tile & 15) == 0) fetch_ids(tile);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = (warp + tile * kAttnWarps) * kTile + u * kUnit;
-        const uint32_t st = ring + ((2 * tile + u) % G::kStages) * G::kUnitBytes;
-        if constexpr (!SMALL_PAGE) {
-          const int32_t id = __shfl_sync(0xffffffffu, ids, 2 * (tile & 15) + u);
-          if (id >= 0) {
-            const uint32_t tok = static_cast<uint32_t>(t_begin + t);
-            const uint8_t* src = base + id * P.cache.block_stride +
-                                 static_cast<int64_t>(P.page_div.mod(tok, P.page_div.div(tok))) * P.cache.token_stride;
-#pragma unroll
-            for (int i = 0; i < G::kChunks; ++i) copy16(st + to[i], src + from[i]);
-            const int n = min(kUnit, count - t);
-            live |= ((1u << n) - 1u) << (16 * u);
-          }
-        } else {  // pages that a unit does not fit into: every row looks up its own
-          const int n = min(kUnit, count - t);
-          int32_t id = -1;
-          if ((lane & 15) < n) {
-            id = table[P.page_div.div(static_cast<uint32_t>(t_begin + t + (lane & 15)))];
+  const int yw = warp % P.y_cta, stream = warp / P.y_cta;
+  const int y = blockIdx.y * P.y_cta + yw;
+  const bool active = y < P.y_total;
+  const int kvh = active ? y / P.chunks : 0;
+  const int h0 = active ? (y - kvh * P.chunks) * kHeads : 0;
+  const int heads = active ? min(kHeads, P.group - h0) : 0;
+  const int head0 = kvh * P.group + h0;  // first query head
+
+  const uint32_t ring = smem_u32(smem) + warp * G::kRingBytes;
+  const int round_tokens = kTile * P.streams;
+  uint32_t phases = 0u;  // of full[warp][0], [1]
+  bool given_up = false;
+
+  while (f < f_end) {
+    const int seq = tokens_of(P, b);
+    const int rounds = rounds_of(seq, P.streams);
+    const int r0 = static_cast<int>(f - first);
+    const int mine = static_cast<int>(min(static_cast<int64_t>(rounds), f_end - first)) - r0;  // tiles of this warp here
+    const bool whole_request = mine == rounds;
+    const int t_begin = r0 * round_tokens + stream * kTile;  // tile i begins at t_begin + i round_tokens
+    const int32_t* table = P.table + b * P.table_stride;
+
+    // Starts the copies of a tile's two units; returns a bit for each of its tokens that counts.
+    int32_t id = -1, at = 0;    // block of the unit that this lane looked up and its first token there
+    uint32_t there = 0u;        // which of the 32 units have a block
+    auto issue = [&](int tile) {
+      if (tile >= mine || !active || given_up) {
+        if constexpr (!TMA) copy_commit();
+        return 0u;
+      }
+      const int t0 = t_begin + tile * round_tokens;
+      const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
+      uint32_t live;
+      if constexpr (TMA) {
+        if ((tile & 15) == 0) {  // the next 32 units, one a lane
+          const int t = t_begin + (tile + (lane >> 1)) * round_tokens + (lane & 1) * kUnit;
+          id = -1;
+          if (tile + (lane >> 1) < mine && t < seq) {
+            const uint32_t col = P.page_div.div(static_cast<uint32_t>(t));
+            at = P.page_div.mod(static_cast<uint32_t>(t), col);
+            id = table[col];
             if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(P.cache.num_blocks)) id = -1;
           }
-          live |= (__ballot_sync(0xffffffffu, id >= 0) & 0xffffu) << (16 * u);
-#pragma unroll
-          for (int i = 0; i < G::kChunks; ++i) {
-            const int c = lane + 32 * i;
-            const int r = (c / G::kChunks) & (kUnit - 1);
-            const int32_t row_id = __shfl_sync(0xffffffffu, id, r);
-            if (row_id >= 0) {
-              const uint32_t tok = static_cast<uint32_t>(t_begin + t + r);
-              copy16(st + to[i], base + row_id * P.cache.block_stride +
-                                     static_cast<int64_t>(P.page_div.mod(tok, P.page_div.div(tok))) *
-                                         P.cache.token_stride +
-                                     from[i]);
-            }
-          }
+          there = __ballot_sync(0xffffffffu, id >= 0);
         }
-      }
-    }
-    copy_commit();
-    return live;
-  };
-
-  // ---- running state: of query head tig (PAIR) or 2 tig + n
-  float m[NH], l[NH], z[NH][NG], w[NH][NG];
-  float acc[NG][4][NH];  // element 32 g + 4 gid + i
-#pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      z[n][g] = w[n][g] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[g][i][n] = 0.f;
-    }
-  }
-
-  live_next = issue(0);
-  for (int tile = 0; tile < mine; ++tile) {
-    const uint32_t live = live_next;
-    live_next = issue(tile + 1);
-    copy_wait<1>();
-    __syncwarp();
-    const uint32_t st = ring + ((2 * tile) % G::kStages) * G::kUnitBytes;
-    const bool whole = live == 0xffffffffu;
-
-    // ---- scores of tokens gid, gid + 8 of both units
-    float s[2][2][NH];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t k0 = st + u * G::kUnitBytes + gid * G::kSmemRow, k1 = k0 + 8 * G::kSmemRow;
-      uint32_t par[2][NG];
-      lds(par[0], k0 + HD / 2);
-      lds(par[1], k1 + HD / 2);
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int n = 0; n < NH; ++n) s[u][r][n] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint32_t x0[1], x1[1];
-        lds(x0, k0 + g * 16 + tig * 4);
-        lds(x1, k1 + g * 16 + tig * 4);
-        const uint32_t a[4] = {x0[0] & 0x0f0f0f0fu, x1[0] & 0x0f0f0f0fu, (x0[0] >> 4) & 0x0f0f0f0fu,
-                               (x1[0] >> 4) & 0x0f0f0f0fu};
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int part = 0; part < (PAIR ? 1 : 2); ++part) mma_e4m3(c, a, bq[part][g][0], bq[part][g][1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float scale = bf_lo(par[r][g]), zero = bf_hi(par[r][g]);
-          if constexpr (PAIR) {
-            s[u][r][0] = fmaf(scale, c[2 * r] + c[2 * r + 1], fmaf(zero, qsum[0][g], s[u][r][0]));
-          } else {
-#pragma unroll
-            for (int n = 0; n < NH; ++n) s[u][r][n] = fmaf(scale, c[2 * r + n], fmaf(zero, qsum[n][g], s[u][r][n]));
-          }
+        const uint32_t two = (there >> (2 * (tile & 15))) & 3u;
+        if (two == 0u) return 0u;
+        if ((lane >> 1) == (tile & 15)) {
+          uint64_t* bar = &full[warp][tile & 1];
+          mbar_arrive_expect_tx(bar, id >= 0 ? G::kUnitBytes : 0);
+          if (id >= 0) copy_unit(st + (lane & 1) * G::kUnitBytes, &map, kvh, at, id, bar);
         }
-      }
-    }
-    // ---- softmax
-    float alpha[NH];
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) s[u][r][n] *= factor[n];
-      if (!whole) {
+        live = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+        if (seq - t0 < kTile) live &= (1u << (seq - t0)) - 1u;
+      } else {  // every row looks its own page up
+        int32_t row_block = -1, row_at = 0;
+        if (t0 + lane < seq) {
+          const uint32_t col = P.page_div.div(static_cast<uint32_t>(t0 + lane));
+          row_at = P.page_div.mod(static_cast<uint32_t>(t0 + lane), col);
+          row_block = table[col];
+          if (static_cast<uint32_t>(row_block) >= static_cast<uint32_t>(P.cache.num_blocks)) row_block = -1;
+        }
+        live = __ballot_sync(0xffffffffu, row_block >= 0);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-            if (!((live >> (16 * u + 8 * r + gid)) & 1u)) s[u][r][n] = -INFINITY;
+          for (int i = 0; i < G::kChunks; ++i) {
+            const int c = lane + 32 * i, v = c >= kUnit * G::kChunks;
+            const int r = c / G::kChunks - (v ? kUnit : 0), piece = c % G::kChunks;
+            const int32_t blk = __shfl_sync(0xffffffffu, row_block, u * kUnit + r);
+            const int32_t off = __shfl_sync(0xffffffffu, row_at, u * kUnit + r);
+            if (blk >= 0)
+              copy16(st + u * G::kUnitBytes + c * 16,
+                     P.cache.base + blk * P.cache.block_stride + (v ? P.cache.outer_stride : 0) +
+                         off * P.cache.token_stride + kvh * P.cache.head_stride + piece * 16);
+          }
+        copy_commit();
       }
-      float top = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
+      return live;
+    };
+    uint32_t live_next = issue(0);
+
+    // ---- q as operands: column gid is head gid / 2, odd columns empty (PAIR), or head gid
+    uint32_t bq[NG][2][2], bz[NZ][2];
+    float factor[NH];
+    {
+      const int h = PAIR ? gid >> 1 : gid;
+      const bool mine_h = h < heads && (!PAIR || (gid & 1) == 0);
+      uint32_t xw[NG][4];
+      float top = 0.f;
+      bool bad = false;
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = fmaxf(m[n], top);
-      const float ref = top == -INFINITY ? 0.f : top;
-      alpha[n] = ex2(m[n] - ref);
-      m[n] = top;
-      l[n] *= alpha[n];
+      for (int g = 0; g < NG; ++g) {
+        int4 w = make_int4(0, 0, 0, 0);
+        if (mine_h)
+          w = *reinterpret_cast<const int4*>(P.q + b * P.q_stride + (head0 + h) * static_cast<int64_t>(HD) +
+                                             g * kGroup + tig * 8);
+        xw[g][0] = w.x, xw[g][1] = w.y, xw[g][2] = w.z, xw[g][3] = w.w;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) z[n][g] *= alpha[n];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          s[u][r][n] = ex2(s[u][r][n] - ref);
-          l[n] += s[u][r][n];
+        for (int k = 0; k < 4; ++k) {
+          top = fmaxf(top, fmaxf(fabsf(bf_lo(xw[g][k])), fabsf(bf_hi(xw[g][k]))));
+          bad |= (xw[g][k] & 0x7f80u) == 0x7f80u || (xw[g][k] & 0x7f800000u) == 0x7f800000u;
         }
+      }
+      int flag = bad;
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        flag |= __shfl_xor_sync(0xffffffffu, flag, o);
+      }
+      const int e = max(exponent(top), -100);  // the largest element comes to [2^14, 2^15)
+      const float up = flag ? 0.f : pow2(14 - e);
+      const float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(P.qscale, 24 + e - 14);
+      float qs[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float x[8];
+        qs[g] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          x[2 * k] = flag ? 0.f : bf_lo(xw[g][k]) * up;
+          x[2 * k + 1] = flag ? 0.f : bf_hi(xw[g][k]) * up;
+          qs[g] += x[2 * k] + x[2 * k + 1];
+        }
+        qs[g] += __shfl_xor_sync(0xffffffffu, qs[g], 1);
+        qs[g] += __shfl_xor_sync(0xffffffffu, qs[g], 2);
+        // register i of a word holds elements i and i + 4, sixteen times too large for odd i
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          bq[g][j][0] = half2(x[2 * j], x[2 * j + 4]);
+          bq[g][j][1] = half2(0.0625f * x[2 * j + 1], 0.0625f * x[2 * j + 5]);
+        }
+      }
+      // sums of q of group tig (+ 4) in the codes' unit 2^-24: three bf16 parts in k slots 2 tig, + 1, + 8 (the fourth: 0)
+#pragma unroll
+      for (int j = 0; j < NZ; ++j) {
+        float s = 0.f;
+#pragma unroll
+        for (int g = 4 * j; g < 4 * j + 4 && g < NG; ++g) s = (g & 3) == tig ? qs[g] : s;
+        s *= pow2(-24);
+        const float s1 = __bfloat162float(__float2bfloat16(s)), s2 = __bfloat162float(__float2bfloat16(s - s1));
+        bz[j][0] = pack2(s1, s2);
+        bz[j][1] = pack2(s - s1 - s2, 0.f);
+      }
+#pragma unroll
+      for (int n = 0; n < NH; ++n) factor[n] = __shfl_sync(0xffffffffu, fac, 8 * tig + 4 * n);
     }
-    // ---- weights times V scales, as operands: PAIR columns are (head, group parity)
-    constexpr int NB = PAIR ? NG / 2 : NG;
-    uint32_t bp[2][NB][2];
+
+    // ---- running state: of query head tig (PAIR) or 2 tig + n
+    float m[NH], l[NH], z[NH][NG];
+    float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24 (16 f 2^-24 for odd i)
+    float vf = pow2(100);  // f; the first tile sets it
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int n = 0; n < NH; ++n) {
+      m[n] = -INFINITY;
+      l[n] = given_up ? __uint_as_float(0x7fc00000u) : 0.f;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        uint32_t par[NG];
-        lds(par, st + u * G::kUnitBytes + (kUnit + gid + 8 * r) * G::kSmemRow + HD / 2);
-        if (!whole && !((live >> (16 * u + 8 * r + gid)) & 1u)) {
+      for (int g = 0; g < NG; ++g) {
+        z[n][g] = 0.f;
 #pragma unroll
-          for (int g = 0; g < NG; ++g) par[g] = 0u;  // what lies behind the last token may be a NaN
+        for (int i = 0; i < 4; ++i) acc[g][i][n] = 0.f;
+      }
+    }
+
+    for (int tile = 0; tile < mine; ++tile) {
+      const uint32_t live = live_next;
+      live_next = issue(tile + 1);
+      if constexpr (!TMA) {
+        copy_wait<1>();
+        __syncwarp();
+      }
+      if (live == 0u) continue;
+      if constexpr (TMA) {
+        const int k = tile & 1;
+        if (!mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs)) given_up = true;
+        if (__any_sync(0xffffffffu, given_up)) {  // leave, when both copies in flight have ended or are given up
+          given_up = true;
+          report_status(&g_kv4_status, kStatusPipelineTimeout);
+          mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
+          if (live_next != 0u) mbar_wait_bounded(&full[warp][k ^ 1], (phases >> (k ^ 1)) & 1u, kWaitNs);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) l[n] = __uint_as_float(0x7fc00000u);
+          break;
         }
-        float ps[NG][NH];
+        phases ^= 1u << k;
+      }
+      const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
+      const bool whole = live == 0xffffffffu;
+
+      // ---- scores of tokens gid, gid + 8 of both units
+      float s[2][2][NH];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t k0 = st + u * G::kUnitBytes + gid * G::kRow, k1 = k0 + 8 * G::kRow;
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NZ; ++j) {
+          uint32_t z0[1], z1[1];  // (lanes without a group of their own meet zeros of bz)
+          lds(z0, k0 + HD / 2 + 16 * j + 4 * (NG < 4 ? tig % NG : tig));
+          lds(z1, k1 + HD / 2 + 16 * j + 4 * (NG < 4 ? tig % NG : tig));
+          z0[0] = __byte_perm(z0[0], 0, 0x3232);
+          z1[0] = __byte_perm(z1[0], 0, 0x3232);
+          mma_bf16(c, z0[0], z1[0], z0[0], z1[0], bz[j][0], bz[j][1], c[0], c[1], c[2], c[3]);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int n = 0; n < NH; ++n) s[u][r][n] = c[2 * r + n];
+        uint32_t par[2][NG];
+        lds(par[0], k0 + HD / 2);
+        lds(par[1], k1 + HD / 2);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float scale = bf_lo(par[g]), mid = fmaf(8.f, scale, bf_hi(par[g]));
+          uint32_t x0[1], x1[1];
+          lds(x0, k0 + g * 16 + tig * 4);
+          lds(x1, k1 + g * 16 + tig * 4);
+          mma_f16(c, code_pair(x0[0], 0), code_pair(x1[0], 0), code_pair(x0[0], 1), code_pair(x1[0], 1), bq[g][0][0],
+                  bq[g][0][1], 0.f, 0.f, 0.f, 0.f);
+          mma_f16(c, code_pair(x0[0], 2), code_pair(x1[0], 2), code_pair(x0[0], 3), code_pair(x1[0], 3), bq[g][1][0],
+                  bq[g][1][1], c[0], c[1], c[2], c[3]);
 #pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            z[n][g] = fmaf(s[u][r][n], mid, z[n][g]);
-            ps[g][n] = s[u][r][n] * scale;
-          }
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int n = 0; n < NH; ++n) s[u][r][n] = fmaf(bf_lo(par[r][g]), c[2 * r + n], s[u][r][n]);
         }
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-          bp[u][k][r] = transpose8x8(PAIR ? pack2(ps[2 * k][0], ps[2 * k + 1][0]) : pack2(ps[k][0], ps[k][NH - 1]));
       }
-    // ---- W = sum p'
+      // ---- softmax
+      float alpha[NH];
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < NH; ++n) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        mma_bf16(c, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, bp[u][k][0], bp[u][k][1]);
-      if constexpr (PAIR) {
-        w[0][2 * k] = fmaf(w[0][2 * k], alpha[0], c[0]);
-        w[0][2 * k + 1] = fmaf(w[0][2 * k + 1], alpha[0], c[1]);
-      } else {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int n = 0; n < NH; ++n) w[n][k] = fmaf(w[n][k], alpha[n], c[n]);
+          for (int r = 0; r < 2; ++r) s[u][r][n] *= factor[n];
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+              if (!((live >> (16 * u + 8 * r + gid)) & 1u)) s[u][r][n] = -INFINITY;
+        }
+        float top = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(m[n], top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        alpha[n] = ex2(m[n] - ref);
+        m[n] = top;
+        l[n] *= alpha[n];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[n][g] *= alpha[n];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            s[u][r][n] = ex2(s[u][r][n] - ref);
+            l[n] += s[u][r][n];
+          }
       }
-    }
-    // ---- acc += sum p' (128 + c): this lane's codes of tokens 2 tig, 2 tig + 1 and those 8 further
-    uint32_t x[2][4][NW];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        lds(x[u][t], st + u * G::kUnitBytes + (kUnit + 2 * tig + (t & 1) + 8 * (t >> 1)) * G::kSmemRow + gid * NW * 4);
-#pragma unroll
-    for (int k = 0; k < NW; ++k) {  // groups 2 k and 2 k + 1
-      uint32_t y[2][2][2];          // [unit][group][tokens 2 tig.. / 8 further]
+      // ---- weights times V scales, as operands: PAIR columns are (head, group parity)
+      uint32_t par[2][2][NG];
+      float top = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          y[u][0][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x5410);
-          y[u][1][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x7632);
+          lds(par[u][r], st + u * G::kUnitBytes + (kUnit + gid + 8 * r) * G::kRow + HD / 2);
+          if (!whole && !((live >> (16 * u + 8 * r + gid)) & 1u)) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) par[u][r][g] = 0u;  // what lies behind the last token may be a NaN
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) top = fmaxf(top, bf_lo(par[u][r][g]));
         }
-      if constexpr (PAIR) {
+      if (__any_sync(0xffffffffu, top * vf > 32768.f)) {  // a larger scale than any before (the first tile's): move f
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float next = pow2(max(13 - exponent(top), -126));
+        const float down = next / vf;
+        vf = next;
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            mma_bf16(c, code_pair(y[u][0][0], i), code_pair(y[u][1][0], i), code_pair(y[u][0][1], i),
-                     code_pair(y[u][1][1], i), bp[u][k][0], bp[u][k][1]);
-          acc[2 * k][i][0] = fmaf(acc[2 * k][i][0], alpha[0], c[0]);
-          acc[2 * k + 1][i][0] = fmaf(acc[2 * k + 1][i][0], alpha[0], c[3]);
-        }
-      } else {
+        for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+          for (int g = 0; g < NG; ++g)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int g = 2 * k + p;
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 4; ++i) acc[g][i][n] *= down;
+      }
+      uint32_t bp[2][NB][2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              mma_bf16(c, code_pair(y[u][p][0], 2 * j), code_pair(y[u][p][0], 2 * j + 1),
-                       code_pair(y[u][p][1], 2 * j), code_pair(y[u][p][1], 2 * j + 1), bp[u][g][0], bp[u][g][1]);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int n = 0; n < NH; ++n) {
-              acc[g][2 * j][n] = fmaf(acc[g][2 * j][n], alpha[n], c[n]);
-              acc[g][2 * j + 1][n] = fmaf(acc[g][2 * j + 1][n], alpha[n], c[2 + n]);
+        for (int r = 0; r < 2; ++r) {
+          float ps[NG][NH];
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            const float pf = s[u][r][n] * vf;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              z[n][g] = fmaf(s[u][r][n], bf_hi(par[u][r][g]), z[n][g]);
+              ps[g][n] = pf * bf_lo(par[u][r][g]);
             }
           }
+#pragma unroll
+          for (int k = 0; k < NB; ++k)
+            bp[u][k][r] = transpose8x8(PAIR ? half2(ps[2 * k][0], ps[2 * k + 1][0]) : half2(ps[k][0], ps[k][NH - 1]));
+        }
+      // ---- acc += sum p' c: this lane's codes of tokens 2 tig, 2 tig + 1 and those 8 further
+      uint32_t x[2][4][NW];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          lds(x[u][t], st + u * G::kUnitBytes + (kUnit + 2 * tig + (t & 1) + 8 * (t >> 1)) * G::kRow + gid * NW * 4);
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {  // groups 2 k and 2 k + 1
+        uint32_t w[2][2][2];          // [unit][group][tokens 2 tig.. / 8 further]: codes i of the pair in nibbles i, i + 4
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            w[u][0][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x5410);
+            w[u][1][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x7632);
+          }
+        if constexpr (PAIR) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float c[4];
+            mma_f16(c, code_pair(w[0][0][0], i), code_pair(w[0][1][0], i), code_pair(w[0][0][1], i),
+                    code_pair(w[0][1][1], i), bp[0][k][0], bp[0][k][1], 0.f, 0.f, 0.f, 0.f);
+            mma_f16(c, code_pair(w[1][0][0], i), code_pair(w[1][1][0], i), code_pair(w[1][0][1], i),
+                    code_pair(w[1][1][1], i), bp[1][k][0], bp[1][k][1], c[0], c[1], c[2], c[3]);
+            acc[2 * k][i][0] = fmaf(acc[2 * k][i][0], alpha[0], c[0]);
+            acc[2 * k + 1][i][0] = fmaf(acc[2 * k + 1][i][0], alpha[0], c[3]);
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // rows 0-7: code 2 j, rows 8-15: code 2 j + 1
+              const int g = 2 * k + p;
+              float c[4];
+              mma_f16(c, code_pair(w[0][p][0], 2 * j), code_pair(w[0][p][0], 2 * j + 1), code_pair(w[0][p][1], 2 * j),
+                      code_pair(w[0][p][1], 2 * j + 1), bp[0][g][0], bp[0][g][1], 0.f, 0.f, 0.f, 0.f);
+              mma_f16(c, code_pair(w[1][p][0], 2 * j), code_pair(w[1][p][0], 2 * j + 1), code_pair(w[1][p][1], 2 * j),
+                      code_pair(w[1][p][1], 2 * j + 1), bp[1][g][0], bp[1][g][1], c[0], c[1], c[2], c[3]);
+#pragma unroll
+              for (int n = 0; n < NH; ++n) {
+                acc[g][2 * j][n] = fmaf(acc[g][2 * j][n], alpha[n], c[n]);
+                acc[g][2 * j + 1][n] = fmaf(acc[g][2 * j + 1][n], alpha[n], c[2 + n]);
+              }
+            }
+        }
       }
+      __syncwarp();
     }
+    if constexpr (!TMA) copy_wait<0>();
     __syncwarp();
-  }
-  copy_wait<0>();
 
-  // ---- sums over the lanes that share a head, then the 4 warps
+    // ---- sums over the lanes that share a head; codes' unit and f out of the sums, zeros' part in
 #pragma unroll
-  for (int n = 0; n < NH; ++n)
+    for (int n = 0; n < NH; ++n) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+      for (int o = 4; o < 32; o <<= 1) {
+        l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) z[n][g] += __shfl_xor_sync(0xffffffffu, z[n][g], o);
-    }
-  __shared__ float red_m[kAttnWarps][kHeads], red_l[kAttnWarps][kHeads];
-  float* red = reinterpret_cast<float*>(smem);  // [warps][heads][HD], in the ring's place
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < NH; ++n) {
-    const int h = NH * tig + n;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float off = fmaf(-136.f, w[n][g], z[n][g]);
-      *reinterpret_cast<float4*>(red + (warp * kHeads + h) * HD + g * kGroup + gid * 4) =
-          make_float4(acc[g][0][n] + off, acc[g][1][n] + off, acc[g][2][n] + off, acc[g][3][n] + off);
-    }
-    if (gid == 0) {
-      red_m[warp][h] = m[n];
-      red_l[warp][h] = l[n];
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * HD; i += kAttnWarps * 32) {
-    const int h = i / HD, d = i - h * HD;
-    float M = -INFINITY, L = 0.f, A = 0.f;
-#pragma unroll
-    for (int k = 0; k < kAttnWarps; ++k) M = fmaxf(M, red_m[k][h]);
-#pragma unroll
-    for (int k = 0; k < kAttnWarps; ++k) {
-      if (red_l[k][h] == 0.f) continue;
-      const float f = exp2f(red_m[k][h] - M);
-      L += f * red_l[k][h];
-      A += f * red[(k * kHeads + h) * HD + d];
-    }
-    if (splits == 1) {
-      P.out[(bh0 + h) * HD + d] = __float2bfloat16(L == 0.f ? 0.f : A / L);
-    } else {
-      const int64_t row = (bh0 + h) * splits + split;
-      P.part_acc[row * HD + d] = A;
-      if (d == 0) {
-        P.part_ml[row * 2] = M;
-        P.part_ml[row * 2 + 1] = L;
+        for (int g = 0; g < NG; ++g) z[n][g] += __shfl_xor_sync(0xffffffffu, z[n][g], o);
       }
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[g][i][n] = fmaf(acc[g][i][n] * (i & 1 ? 1048576.f : 16777216.f), 1.f / vf, z[n][g]);
+    }
+    // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
+    if (P.streams > 1) {
+      constexpr int kVals = NH * (2 + 4 * NG);
+      float* red = reinterpret_cast<float*>(smem) + warp * kVals * 32 + lane;
+      __syncthreads();
+      if (stream > 0) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          red[(2 * n) * 32] = m[n];
+          red[(2 * n + 1) * 32] = l[n];
+#pragma unroll
+          for (int k = 0; k < 4 * NG; ++k) red[(2 * NH + n * 4 * NG + k) * 32] = acc[k / 4][k % 4][n];
+        }
+      }
+      __syncthreads();
+      if (stream == 0) {
+        for (int t = 1; t < P.streams; ++t) {
+          const float* o = red + t * P.y_cta * kVals * 32;
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            const float mo = o[(2 * n) * 32], lo = o[(2 * n + 1) * 32];
+            const float top = fmaxf(m[n], mo);
+            const float f0 = l[n] == 0.f ? 0.f : exp2f(m[n] - top), f1 = lo == 0.f ? 0.f : exp2f(mo - top);
+            m[n] = top;
+            l[n] = f0 * l[n] + f1 * lo;
+#pragma unroll
+            for (int k = 0; k < 4 * NG; ++k)
+              acc[k / 4][k % 4][n] = f0 * acc[k / 4][k % 4][n] + f1 * o[(2 * NH + n * 4 * NG + k) * 32];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // ---- to the output, or to this CTA's slot of partial results
+    if (stream == 0 && active) {
+      const int64_t slot_row = (static_cast<int64_t>(blockIdx.x) * 2 + (f == f_begin ? 0 : 1)) * P.hq + head0;
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        const int h = NH * tig + n;
+        if (h >= heads) continue;
+        const float r = whole_request ? (l[n] == 0.f ? 0.f : 1.f / l[n]) : 1.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const int d = g * kGroup + gid * 4;
+          if (whole_request)
+            *reinterpret_cast<uint2*>(P.out + (static_cast<int64_t>(b) * P.hq + head0 + h) * HD + d) =
+                make_uint2(pack2(acc[g][0][n] * r, acc[g][1][n] * r), pack2(acc[g][2][n] * r, acc[g][3][n] * r));
+          else
+            *reinterpret_cast<float4*>(P.part_acc + (slot_row + h) * HD + d) =
+                make_float4(acc[g][0][n], acc[g][1][n], acc[g][2][n], acc[g][3][n]);
+        }
+        if (!whole_request && gid == 0) {
+          P.part_ml[(slot_row + h) * 2] = m[n];
+          P.part_ml[(slot_row + h) * 2 + 1] = l[n];
+        }
+      }
+      if (r0 == 0 && y == 0 && lane == 0) P.first[b] = first;
+    }
+    f = first + r0 + mine;
+    if (r0 + mine == rounds) {
+      first += rounds;
+      ++b;
     }
   }
-  if (splits == 1 || P.counters == nullptr) return;
-  __shared__ unsigned int ticket;
-  __threadfence();
-  __syncthreads();
-  unsigned int* counter = &P.counters[static_cast<int64_t>(b) * gridDim.y + blockIdx.y];
-  if (threadIdx.x == 0) ticket = atomicAdd(counter, 1u);
-  __syncthreads();
-  if (ticket != static_cast<unsigned int>(splits - 1)) return;
-  __threadfence();
-  for (int i = threadIdx.x; i < heads * HD; i += kAttnWarps * 32) merge_row<HD>(P, bh0 + i / HD, splits, i % HD);
-  if (threadIdx.x == 0) *counter = 0u;
 }
 
-template <int HD, bool PAIR, bool SMALL_PAGE>
-cudaError_t launch_decode_kernel(const AttnParams& P, dim3 grid, cudaStream_t stream) {
-  auto kernel = kv4_decode_kernel<HD, PAIR, SMALL_PAGE>;
-  constexpr int kSmem = Geometry<HD>::kSmem > kAttnWarps * kHeads * HD * 4 ? Geometry<HD>::kSmem
-                                                                          : kAttnWarps * kHeads * HD * 4;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+// How a launch is laid out: (KV head, chunk) pairs and streams a CTA, CTAs along the work.
+struct Plan {
+  int chunks, y_total, y_cta, y_ctas, streams, ctas;
+};
+inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, int ctas, int sm_count) {
+  Plan p{};
+  p.chunks = (hq / hkv + kHeads - 1) / kHeads;
+  p.y_total = hkv * p.chunks;
+  // As many KV heads a CTA as it has warps, unless requests are so few that each would be cut into more than 32
+  // parts: streams of tokens are merged within a CTA, parts by the second kernel (131,072 tokens of one request,
+  // 8 KV heads: 296 parts of 8 heads 69 us, 37 of one head 44 us).
+  for (p.y_cta = (p.y_total + (p.y_total - 1) / kMaxWarps) / ((p.y_total - 1) / kMaxWarps + 1);; --p.y_cta) {
+    p.y_ctas = (p.y_total + p.y_cta - 1) / p.y_cta;
+    p.streams = kMaxWarps / p.y_cta;
+    // registers allow 16 warps an SM (8 with 256 elements a head)
+    const int per_sm = std::max(1, (hd == 256 ? 8 : 16) / (p.y_cta * p.streams));
+    p.ctas = ctas > 0 ? ctas : std::max(1, sm_count * per_sm / p.y_ctas);
+    if (p.ctas / batch < 32 || p.y_cta == 1) break;
+  }
+  const int64_t rounds = (max_tokens + kTile * p.streams - 1) / (kTile * p.streams);
+  p.ctas = static_cast<int>(std::min<int64_t>(p.ctas, std::max<int64_t>(1, (batch * rounds + kMinRounds - 1) / kMinRounds)));
+  return p;
+}
+
+// The pool as a tensor of bytes [block][K / V][token][head][row], boxes of a unit's rows of one head.
+inline bool make_map(CUtensorMap* map, const Cache& c, int row) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? p : nullptr);
+  }();
+  if (!fn || c.num_blocks < 1) return false;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(row), static_cast<cuuint64_t>(c.heads),
+                              static_cast<cuuint64_t>(c.page), 2, static_cast<cuuint64_t>(c.num_blocks)};
+  // a dimension of one may come with any stride
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(c.heads > 1 ? c.head_stride : row),
+                                 static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.outer_stride),
+                                 static_cast<cuuint64_t>(c.num_blocks > 1 ? c.block_stride : row)};
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(row), 1, kUnit, 2, 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+template <int HD, bool PAIR, bool TMA>
+cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, const Plan& plan, cudaStream_t stream) {
+  auto kernel = kv4_decode_kernel<HD, PAIR, TMA>;
+  const int warps = plan.y_cta * plan.streams;
+  constexpr int kVals = (PAIR ? 1 : 2) * (2 + 4 * (HD / kGroup));  // merging streams, in the ring's place
+  const int smem = warps * std::max(Geometry<HD>::kRingBytes, kVals * 128);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<grid, kAttnWarps * 32, kSmem, stream>>>(P);
+  kernel<<<dim3(plan.ctas, plan.y_ctas), warps * 32, smem, stream>>>(P, map);
   return cudaGetLastError();
 }
 
 template <int HD>
-cudaError_t launch_decode_hd(const AttnParams& P, int batch, int splits, cudaStream_t stream) {
-  const int chunks = (P.group + kHeads - 1) / kHeads;
-  const int64_t y = static_cast<int64_t>(P.cache.heads) * chunks;
-  if (y > 65535) return cudaErrorInvalidValue;
-  const dim3 grid(splits, static_cast<unsigned>(y), batch);
-  const bool small = P.cache.page % kUnit != 0;
+cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t stream) {
+  CUtensorMap map{};
+  const bool tma = P.cache.page % kUnit == 0 && make_map(&map, P.cache, row_bytes(HD));
   cudaError_t e;
   if (P.group <= 4)
-    e = small ? launch_decode_kernel<HD, true, true>(P, grid, stream)
-              : launch_decode_kernel<HD, true, false>(P, grid, stream);
+    e = tma ? launch_decode_kernel<HD, true, true>(P, map, plan, stream)
+            : launch_decode_kernel<HD, true, false>(P, map, plan, stream);
   else
-    e = small ? launch_decode_kernel<HD, false, true>(P, grid, stream)
-              : launch_decode_kernel<HD, false, false>(P, grid, stream);
-  if (e != cudaSuccess || splits == 1 || P.counters != nullptr) return e;
-  kv4_merge_kernel<HD><<<static_cast<unsigned>(batch) * P.hq, HD, 0, stream>>>(P, splits);
-  return cudaGetLastError();
+    e = tma ? launch_decode_kernel<HD, false, true>(P, map, plan, stream)
+            : launch_decode_kernel<HD, false, false>(P, map, plan, stream);
+  if (e != cudaSuccess || plan.ctas == 1) return e;
+  cudaLaunchConfig_t cfg{};
+  // a head a CTA while that leaves SMs free for it
+  const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 1024 ? 1 : kMergeWarps;
+  cfg.gridDim = dim3((P.hq + heads_cta - 1) / heads_cta, P.batch);
+  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD>, P, heads_cta);
 }
 
-inline cudaError_t launch_decode(const AttnParams& P, int batch, int hd, int splits, cudaStream_t stream) {
+inline cudaError_t launch_decode(const AttnParams& P, int hd, const Plan& plan, cudaStream_t stream) {
   switch (hd) {
-    case 64: return launch_decode_hd<64>(P, batch, splits, stream);
-    case 128: return launch_decode_hd<128>(P, batch, splits, stream);
-    case 256: return launch_decode_hd<256>(P, batch, splits, stream);
+    case 64: return launch_decode_hd<64>(P, plan, stream);
+    case 128: return launch_decode_hd<128>(P, plan, stream);
+    case 256: return launch_decode_hd<256>(P, plan, stream);
     default: return cudaErrorInvalidValue;
   }
 }

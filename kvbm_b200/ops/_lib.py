@@ -140,11 +140,13 @@ _SIGS = {
         _INT,
         [_VP, _I64, _I64, _I64, _I64, _INT, _INT, _INT, _INT, _VP, _I64, _VP, _VP, _VP],
     ),
+    "kvbm_paged_decode_attn_kv4_plan": (_INT, [_INT, _INT, _INT, _INT, _I64, _INT, _INT, C.POINTER(_I64)]),
     "kvbm_paged_decode_attn_kv4": (
         _INT,
         [_VP, _I64, _VP, _I64, _I64, _I64, _I64, _INT, _INT, _VP, _I64, _INT, _VP, _INT, _INT, _INT, _INT, _F32, _INT,
-         _VP, _VP, _VP, _VP, _VP],
+         _INT, _VP, _VP, _VP],
     ),
+    "kvbm_kv4_status": (_INT, [_INT]),
     "kvbm_skinny_gemm": (_INT, [_VP, _INT, _VP, _INT, _VP, _INT, _INT, _INT, _INT, _INT, _VP, _VP, _VP]),
     "kvbm_skinny_gemm_ctas": (_INT, []),
     "kvbm_skinny_gemm_set_pdl": (_INT, [_INT]),
@@ -193,7 +195,7 @@ _KERNELS_PER_CALL = {
     "kvbm_rope_kv_push": 1, "kvbm_rope_kv_write_qout": 1, "kvbm_rope_kv_push_heads": 1,
     "kvbm_silu_mul": 1, "kvbm_paged_decode_attn": 2, "kvbm_paged_decode_attn_fused": 1, "kvbm_paged_decode_attn_simt": 2,
     "kvbm_batch_tables": 1, "kvbm_slot_map": 1, "kvbm_qk_norm_rope_kv_write": 1, "kvbm_kv4_gather": 1,
-    "kvbm_paged_decode_attn_kv4": 1,
+    "kvbm_paged_decode_attn_kv4": 2,
     "kvbm_skinny_gemm": 1, "kvbm_kv_multicast": 1, "kvbm_signal_multicast": 1,
 }
 _launches = 0

@@ -13,7 +13,8 @@ tokens, such a slot is not written and reads as zeros.
 
 from __future__ import annotations
 
-import math
+import ctypes as C
+import functools
 
 import torch
 
@@ -132,24 +133,36 @@ def kv4_gather(kv: torch.Tensor, slots: torch.Tensor, *, k_out: torch.Tensor | N
     return k_out, v_out
 
 
-def kv4_decode_splits(batch: int, hq: int, hkv: int, max_tokens: int, sm_count: int = 148) -> int:
-    """KV ranges :func:`paged_decode_attn_kv4` cuts each sequence into."""
-    groups = max(1, batch * hkv * math.ceil(hq / hkv / 8))
-    return max(1, min(math.ceil(max_tokens / 64), math.ceil(4 * sm_count / groups)))
+@functools.lru_cache(maxsize=256)
+def _decode_plan(batch: int, hq: int, hkv: int, hd: int, max_tokens: int, ctas: int, device: int) -> tuple:
+    """(floats of scratch, SMs) of a launch of these sizes."""
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    out = (C.c_int64 * 2)()
+    _lib.check(_lib.load().kvbm_paged_decode_attn_kv4_plan(batch, hq, hkv, hd, min(max_tokens, 2 ** 31 - 1), ctas, sms,
+                                                           out), "kvbm_paged_decode_attn_kv4_plan")
+    return int(out[0]), sms
+
+
+def kv4_decode_scratch(batch: int, hq: int, hkv: int, head_dim: int, max_tokens: int, ctas: int = 0,
+                       device=None) -> int:
+    """Floats of scratch that :func:`paged_decode_attn_kv4` takes for these sizes (``max_tokens``: the block
+    table's width in tokens)."""
+    dev = torch.device(device if device is not None else "cuda")
+    return _decode_plan(batch, hq, hkv, head_dim, max_tokens, ctas,
+                        dev.index if dev.index is not None else torch.cuda.current_device())[0]
 
 
 def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                          softmax_scale: float, *, splits: int | None = None, scratch: torch.Tensor | None = None,
-                          counters: torch.Tensor | None = None, out: torch.Tensor | None = None,
-                          stream=None) -> torch.Tensor:
+                          softmax_scale: float, *, ctas: int = 0, scratch: torch.Tensor | None = None,
+                          out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Attention of one token per request over a 4-bit paged cache. q: bf16 [B, Hq, hd]; returns the same.
 
     Hq is a multiple of the cache's heads. ``block_table`` (int32 [B, max_blocks]) and ``seq_lens`` (int32 [B])
     as for the 16-bit kernel; a length beyond the table counts as the table's, one of 0 or less gives zeros, and a
-    page whose id is outside the pool holds no tokens. ``splits`` (by default from the batch and the table's
-    width) KV ranges run in parallel; their partial results need ``scratch`` (fp32, B * Hq * splits * (hd + 2);
-    made here if not given). ``counters`` (int32, at least B * Hq zeros; zero again afterwards) lets the last CTA
-    merge them in the same launch. Launches that may overlap need a scratch and counters each.
+    page whose id is outside the pool holds no tokens. The work is cut evenly over ``ctas`` CTAs (0: as many as
+    the GPU holds at a time), whatever the lengths; results of requests that several CTAs share go through
+    ``scratch`` (fp32, :func:`kv4_decode_scratch` entries; made here if not given, nothing in it outlives the
+    call). Launches that may overlap need a scratch each.
     """
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be bf16 [B, Hq, hd]")
@@ -169,35 +182,34 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
         raise ValueError(f"block_table must be int32 [{B}, max_blocks] with unit inner stride on {dev}")
     _vec(seq_lens, "seq_lens", torch.int32, B, dev)
     max_blocks = block_table.shape[1]
-    if splits is None:
-        splits = kv4_decode_splits(B, hq, hkv, max_blocks * kv.shape[2])
-    elif splits < 1:
-        raise ValueError("splits must be at least 1")
-    rows = B * hq * splits
-    if counters is not None and (counters.dtype != torch.int32 or counters.numel() < B * hq
-                                 or counters.device != dev or not counters.is_contiguous()):
-        raise ValueError(f"counters must be int32 with at least {B * hq} entries on {dev}")
-    if scratch is not None and (scratch.dtype != torch.float32 or scratch.numel() < rows * (hd + 2)
-                                or scratch.device != dev or not scratch.is_contiguous()):
-        raise ValueError(f"scratch must be fp32 with at least {rows * (hd + 2)} entries on {dev}")
+    if ctas < 0:
+        raise ValueError("ctas must not be negative")
+    if scratch is not None and (scratch.dtype != torch.float32 or scratch.device != dev
+                                or not scratch.is_contiguous() or scratch.data_ptr() % 16):
+        raise ValueError(f"scratch must be 16-byte aligned fp32 on {dev}")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
                             or out.device != dev or out.data_ptr() % 16):
         raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} on {dev}")
     with _lib.on_device(dev, stream) as st:
         if out is None:
             out = torch.empty(B, hq, hd, dtype=q.dtype, device=dev)
-        acc = ml = None
-        if splits > 1:
-            if scratch is None:
-                scratch = torch.empty(rows * (hd + 2), dtype=torch.float32, device=dev)
-            acc = scratch.data_ptr()
-            ml = acc + rows * hd * 4
+        if B == 0:
+            return out
+        need, sms = _decode_plan(B, hq, hkv, hd, max_blocks * kv.shape[2], ctas, dev.index)
+        if scratch is None:
+            scratch = torch.empty(need, dtype=torch.float32, device=dev)
+        elif scratch.numel() < need:
+            raise ValueError(f"scratch holds {scratch.numel()} floats, {need} are needed")
         _lib.call("kvbm_paged_decode_attn_kv4", q.data_ptr(), q.stride(0), *cache, block_table.data_ptr() or None,
-                  block_table.stride(0), max_blocks, seq_lens.data_ptr(), B, hq, hkv, hd, softmax_scale, splits, acc,
-                  ml, counters.data_ptr() if counters is not None else None, out.data_ptr(), st)
-        if splits > 1 and counters is None:
-            _lib.count_launches(1)  # the merge
+                  block_table.stride(0), max_blocks, seq_lens.data_ptr(), B, hq, hkv, hd, softmax_scale, ctas, sms,
+                  scratch.data_ptr(), out.data_ptr(), st)
     return out
+
+
+def kv4_status(reset: bool = True) -> int:
+    """0, or the error a :func:`paged_decode_attn_kv4` launch recorded (3: a wait for a copy timed out; its results
+    are NaN). Synchronizes."""
+    return int(_lib.load().kvbm_kv4_status(1 if reset else 0))
 
 
 # ------------------------------------------------------------- rows on the host

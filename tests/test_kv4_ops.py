@@ -113,9 +113,8 @@ def _attn_args(**kw):
     (dict(block_table=torch.zeros(2, 3, dtype=torch.int64)), "block_table"),
     (dict(block_table=torch.zeros(3, 2, dtype=torch.int32).t()), "block_table"),
     (dict(seq_lens=torch.zeros(3, dtype=torch.int32)), "seq_lens"),
-    (dict(splits=0), "splits"),
-    (dict(counters=torch.zeros(3, dtype=torch.int32)), "counters"),
-    (dict(splits=2, scratch=torch.zeros(10)), "scratch"),
+    (dict(ctas=-1), "ctas"),
+    (dict(scratch=torch.zeros(10, dtype=torch.float64)), "scratch"),
     (dict(out=torch.zeros(2, 8, 64, dtype=BF)), "out"),
     ({}, "CUDA tensors"),
 ])

@@ -314,34 +314,36 @@ def _check_attn(got, q, vals, scale, **kw):
     assert (err <= bound).all(), (float((err - bound).max()), float(err.max()))
 
 
-@pytest.mark.parametrize("counters", [False, True])
-@pytest.mark.parametrize("lens,hkv,group,hd,page,order,splits", [
-    ([1], 1, 1, 64, 16, "nhd", None),
+@pytest.mark.parametrize("lens,hkv,group,hd,page,order,ctas", [
+    ([1], 1, 1, 64, 16, "nhd", 0),
     ([1, 2, 15, 16, 17, 31, 33], 2, 4, 128, 16, "nhd", 1),
     ([0, 300, 5, 64, 65], 2, 7, 64, 32, "hnd", 3),           # an empty request
     ([0, 0], 1, 3, 128, 16, "nhd", 2),                        # nothing but empty ones
-    ([129, 1000], 3, 5, 128, 64, "hnd", None),
+    ([129, 1000], 3, 5, 128, 64, "hnd", 0),
     ([77, 700, 3], 1, 8, 256, 16, "nhd", 5),
     ([40, 41], 2, 1, 256, 1, "nhd", 2),                       # pages of one token
     ([100, 513], 2, 2, 128, 8, "hnd", 4),                     # pages that end inside a tile
     ([257, 90], 1, 16, 64, 16, "nhd", 3),                     # more query heads than a CTA takes
     ([333, 47], 1, 13, 128, 16, "hnd", 7),
-    ([2100], 8, 4, 128, 16, "nhd", 40),                       # more ranges than pages for some
+    ([2100], 8, 4, 128, 16, "nhd", 400),                       # more CTAs than it has work for
     ([5], 4, 6, 64, 128, "nhd", 9),
+        ([3000, 2500], 1, 4, 64, 16, "nhd", 0),                   # 8 streams of tokens, many CTAs a request
+        ([700, 0, 900, 1], 3, 3, 128, 32, "hnd", 2),              # CTAs that begin and end inside requests
+        ([150] * 9, 12, 2, 64, 16, "nhd", 5),                     # more KV heads than a CTA has warps
+        ([6000], 5, 4, 128, 16, "nhd", 0),
 ])
-def test_paged_decode_attention(lens, hkv, group, hd, page, order, splits, counters):
+def test_paged_decode_attention(lens, hkv, group, hd, page, order, ctas):
     B = len(lens)
     kv, table, vals = _filled(B, lens, hkv, hd, page, order, seed=sum(lens) + hd)
     q = 2 * torch.randn(B, hkv * group, hd, device="cuda", generator=_gen(9))
     q = q.to(BF)
-    c = torch.zeros(B * hkv * group, dtype=torch.int32, device="cuda") if counters else None
     seq = _i32(lens)
-    for _ in range(2):  # the tickets are left zero
-        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 1 / math.sqrt(hd), splits=splits, counters=c)
+    for _ in range(2):  # a call leaves nothing to the next
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 1 / math.sqrt(hd), ctas=ctas)
         _check_attn(got, q, vals, 1 / math.sqrt(hd))
-        assert c is None or not c.any()
     for b, n in enumerate(lens):
         assert n or not got[b].any()
+    assert kv4_ops.kv4_status() == 0
 
 
 def test_attention_strided_query_table_and_caller_buffers():
@@ -351,9 +353,9 @@ def test_attention_strided_query_table_and_caller_buffers():
     q = wide[:, :8]
     big = torch.zeros(3, table.shape[1] + 5, dtype=torch.int32, device="cuda")
     big[:, : table.shape[1]] = table
-    scratch = torch.full((3 * 8 * 4 * (hd + 2),), math.nan, device="cuda")
+    scratch = torch.full((kv4_ops.kv4_decode_scratch(3, 8, hkv, hd, table.shape[1] * page, 4),), math.nan, device="cuda")
     out = torch.empty(3, 8, hd, dtype=BF, device="cuda")
-    got = kv4_ops.paged_decode_attn_kv4(q, kv, big[:, : table.shape[1]], _i32(lens), 0.1, splits=4, scratch=scratch, out=out)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, big[:, : table.shape[1]], _i32(lens), 0.1, ctas=4, scratch=scratch, out=out)
     assert got.data_ptr() == out.data_ptr()
     _check_attn(got, q, vals, 0.1)
     # a table wider than the sequences need, and lengths beyond the table's width
@@ -373,7 +375,7 @@ def test_attention_pages_outside_the_pool_hold_no_tokens():
     keep = [torch.arange(64, device="cuda") // 16 != 1, torch.arange(64, device="cuda") // 16 != 0,
             torch.zeros(64, dtype=torch.bool, device="cuda")]
     q = torch.randn(3, 8, hd, device="cuda", generator=_gen(2)).to(BF)
-    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.2, splits=2)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.2, ctas=2)
     _check_attn(got, q, [tuple(x[m] for x in v) for v, m in zip(vals, keep)], 0.2)
     assert not got[2].any()
 
@@ -403,8 +405,8 @@ def test_attention_one_token_far_above_many():
     q = torch.zeros(1, 1, hd, device="cuda", dtype=BF)
     q[0, 0, 0] = 1.0
     vals = [_values(rk, rv)]
-    for splits in (1, 8):
-        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, splits=splits)
+    for ctas in (1, 8):
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, ctas=ctas)
         _check_attn(got, q, vals, 1.0)
 
 
@@ -414,7 +416,7 @@ def test_attention_poison_shows_only_where_it_is():
     blk = int(table[0, 1])
     kv[blk, 0, 3, 1] = 255  # one K row of request 0, KV head 1
     q = torch.randn(2, 4, hd, device="cuda", generator=_gen(4)).to(BF)
-    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, splits=3)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, ctas=3)
     assert got[0, 2:].isnan().all()
     want, _ = _attn64(q, vals, 0.1)
     assert got[0, :2].isfinite().all() and got[1].isfinite().all()
@@ -438,7 +440,7 @@ def test_offsets_beyond_32_bits():
     kg, vg = kv4_ops.kv4_gather(kv, slots)
     assert torch.equal(vg, kv4_ops.unpack_rows(kv4_ops.pack_rows(x[:, 2 * hkv:], True), True).to(BF))
     vals = [_values(kv4_ops.pack_rows(k, False), kv4_ops.pack_rows(x[:, 2 * hkv:], True))]
-    got = kv4_ops.paged_decode_attn_kv4(q[29:], kv, _i32([[far, 1]]), _i32([30]), 0.1, splits=2)
+    got = kv4_ops.paged_decode_attn_kv4(q[29:], kv, _i32([[far, 1]]), _i32([30]), 0.1, ctas=2)
     _check_attn(got, q[29:], vals, 0.1)
 
 
@@ -472,7 +474,7 @@ def _steps(kv, cs, prompt, owned, ids, T, x, y, w, hq=8, hkv=2, hd=128, page=16)
     slots = table_ops.slot_map(t.block_table, pos, page=page)
     q2 = torch.empty(B, hq, hd, dtype=BF, device="cuda")
     kv4_ops.qk_norm_rope_kv_write(y, pos, cs, hq, hkv, kv, slots, q_weight=w[0], k_weight=w[1], q_out=q2)
-    out = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, pos + 1, 1 / math.sqrt(hd), splits=2)
+    out = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, pos + 1, 1 / math.sqrt(hd), ctas=2)
     return t, q2, out
 
 
@@ -522,7 +524,7 @@ def test_operators_together_captured_and_on_another_stream():
     s = torch.cuda.Stream()
     t, q1, q2, slots = step(stream=s)
     got = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, _i32([n + 1 for n in prompt]), 1 / math.sqrt(128),
-                                        splits=2, stream=s.cuda_stream)
+                                        ctas=2, stream=s.cuda_stream)
     s.synchronize()
     assert torch.equal(got, want)
     kv.zero_()
@@ -531,7 +533,7 @@ def test_operators_together_captured_and_on_another_stream():
     torch.cuda.synchronize()
     with torch.cuda.graph(graph):
         t, q1, q2, slots = step()
-        got = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, seq, 1 / math.sqrt(128), splits=2)
+        got = kv4_ops.paged_decode_attn_kv4(q2, kv, t.block_table, seq, 1 / math.sqrt(128), ctas=2)
     for _ in range(2):
         kv.zero_()
         got.zero_()

@@ -9,6 +9,7 @@
 
 using namespace kvbm;
 using kvbm::kv4::Cache;
+using kvbm::kv4::f32x2;
 
 namespace {
 
@@ -23,9 +24,17 @@ constexpr int kThreads = 256;
 // all in fp32 and rounded to bf16 once. The cache takes that bf16 k and the bf16
 // v, so quantising a 16-bit cache later gives the same codes.
 //
-// A row of HD elements is held by HD/8 lanes, 16 bytes each. The rotation
-// partner's input (not its normalised value) comes by shuffle: both lanes know
-// the row's 1/rms, so exchanging 4 packed registers does.
+// A row of HD elements is held by HD/16 lanes, each with 8 elements of the first
+// half and the 8 that lie HD/2 behind them, so with rot = HD both elements of a
+// rotation are in one lane (with a smaller rot the other comes by shuffle), and
+// a warp takes 512 / HD rows a step. With w folded into the cosines and sines
+// once a token, out = 1/rms (x (w cos) - x' (w' sin)) costs three multiplies an
+// element, done in pairs.
+// What bounds it is HBM for a prefill (the rows go in and out once), nearly
+// matched by the instructions of the norm, the rotation and the quantising: hence
+// the packed arithmetic, and the next step's loads in flight under each step. For
+// a decode step it is the latency of one token, so there a token's rows are
+// spread over warps. Rows are taken by kind (q, k, v), which keeps branches uniform.
 // ---------------------------------------------------------------------------
 struct WriteParams {
   __nv_bfloat16* qkv;
@@ -39,133 +48,231 @@ struct WriteParams {
   float eps;
   const int64_t* slots;
   Cache cache;
-  FastDiv page_div, heads_div;
+  int steps_q, steps_kv, steps_item;  // steps of a token's q rows, of its k (v) rows, of one warp
+  FastDiv items_div;                  // divides by the items of a token
   __nv_bfloat16* q_out;
   __nv_bfloat16* k_out;
 };
 
-template <int HD, bool KV4>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
-  constexpr int L = HD / 8;  // lanes a row
-  const int H = P.hq + 2 * P.hkv;
-  const int l = threadIdx.x % L;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;
-  const int64_t t = item / H;
-  const int h = static_cast<int>(item - t * H);
-  const bool live = t < P.tokens;
-  const int32_t pos = live ? P.positions[t] : -1;
-  const bool ok = pos >= 0 && pos < P.max_pos;  // a token outside the table is left alone
-  const bool is_q = h < P.hq, is_v = h >= P.hq + P.hkv;
-  __nv_bfloat16* row = P.qkv + t * P.qkv_stride + static_cast<int64_t>(h) * HD + 8 * l;
-  int4 x4 = make_int4(0, 0, 0, 0);
-  if (ok) x4 = *reinterpret_cast<const int4*>(row);
-  uint32_t x[4] = {(uint32_t)x4.x, (uint32_t)x4.y, (uint32_t)x4.z, (uint32_t)x4.w};
+// Read once, possibly written in place later: past L1, but not by the read-only path.
+__device__ __forceinline__ int4 load_once(const void* p) {
+  int4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void words(uint32_t (&x)[4], int4 v) { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
 
-  float ss = 0.f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float a = kv4::bf_lo(x[k]), b = kv4::bf_hi(x[k]);
-    ss = fmaf(a, a, fmaf(b, b, ss));
-  }
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const int half = P.rot / 16;  // lanes that hold one half of the rotated elements
-  const int partner = l < half ? l + half : l < 2 * half ? l - half : l;
-  uint32_t xp[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) xp[k] = __shfl_sync(0xffffffffu, x[k], partner, L);
+enum Kind { kQ, kK, kV };
 
-  if (ok && !is_v) {
-    const __nv_bfloat16* w = is_q ? P.q_weight : P.k_weight;
-    float inv = 1.f;
-    uint32_t wm[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, wp[4] = {wm[0], wm[0], wm[0], wm[0]};
-    if (w != nullptr) {
-      inv = rsqrtf(ss / HD + P.eps);
-      const int4 a = reinterpret_cast<const int4*>(w)[l], b = reinterpret_cast<const int4*>(w)[partner];
-      wm[0] = a.x, wm[1] = a.y, wm[2] = a.z, wm[3] = a.w;
-      wp[0] = b.x, wp[1] = b.y, wp[2] = b.z, wp[3] = b.w;
+template <int HD, bool KV4, bool FULL, Kind KIND>
+__device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int begin, int end, int32_t pos,
+                                           uint8_t* cache_row) {
+  constexpr int L = HD / 16, R = 32 / L;  // lanes a row, rows a step
+  const int lane = threadIdx.x & 31, l = lane % L, r = lane / L;
+  const int rows = KIND == kQ ? P.hq : P.hkv;
+  const int head0 = KIND == kQ ? 0 : KIND == kK ? P.hq : P.hq + P.hkv;
+  __nv_bfloat16* src = P.qkv + t * P.qkv_stride + static_cast<int64_t>(head0) * HD + 8 * l;
+  int4 next[2];  // the next step's rows, in flight (two steps ahead cost registers: 24 warps an SM are worth more)
+  auto load = [&](int step) {
+    const int h = step * R + r;
+    next[0] = next[1] = make_int4(0, 0, 0, 0);
+    if (step < end && h < rows) {
+      next[0] = load_once(src + static_cast<int64_t>(h) * HD);
+      next[1] = load_once(src + static_cast<int64_t>(h) * HD + HD / 2);
     }
-    float c[8], s[8];
-    if (l < 2 * half) {
-      const float* cs = P.cos_sin + static_cast<int64_t>(pos) * P.rot + (l < half ? l : l - half) * 8;
-      const float sign = l < half ? -1.f : 1.f;
+  };
+  load(begin);
+
+  // Unit i of this lane (8 elements): out = x cw[i] + x' sw[i], x' the unit `other[i]` of the row.
+  f32x2 cw[2][4], sw[2][4];
+  int other[2];
+  const __nv_bfloat16* w = KIND == kQ ? P.q_weight : P.k_weight;
+  if constexpr (KIND != kV) {
+    const int half = FULL ? L : P.rot / 16;  // units that hold one half of the rotated elements
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        c[k] = cs[k];
-        s[k] = sign * cs[P.rot / 2 + k];
+    for (int i = 0; i < 2; ++i) {
+      const int u = l + i * L;
+      other[i] = u < half ? u + half : u < 2 * half ? u - half : u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) cw[i][k] = kv4::make2(1.f, 1.f), sw[i][k] = 0;
+      if (FULL || u < 2 * half) {
+        const float* cs = P.cos_sin + static_cast<int64_t>(pos) * (FULL ? HD : P.rot) + (u < half ? u : u - half) * 8;
+        const float sign = u < half ? -1.f : 1.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float4 a = *reinterpret_cast<const float4*>(cs + 4 * k);
+          const float4 b = *reinterpret_cast<const float4*>(cs + 8 * half + 4 * k);
+          cw[i][2 * k] = kv4::make2(a.x, a.y), cw[i][2 * k + 1] = kv4::make2(a.z, a.w);
+          sw[i][2 * k] = kv4::make2(sign * b.x, sign * b.y), sw[i][2 * k + 1] = kv4::make2(sign * b.z, sign * b.w);
+        }
       }
-    } else {
+      if (w != nullptr) {
+        uint32_t wm[4], wp[4];
+        words(wm, reinterpret_cast<const int4*>(w)[u]);
+        words(wp, reinterpret_cast<const int4*>(w)[other[i]]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) c[k] = 1.f, s[k] = 0.f;
+        for (int k = 0; k < 4; ++k) {
+          cw[i][k] = kv4::mul2(cw[i][k], kv4::widen(wm[k]));
+          sw[i][k] = kv4::mul2(sw[i][k], kv4::widen(wp[k]));
+        }
+      }
     }
+  }
+  for (int step = begin; step < end; ++step) {
+    const int h = step * R + r;
+    uint32_t x[2][4];
+    words(x[0], next[0]);
+    words(x[1], next[1]);
+    load(step + 1);
+    if constexpr (KIND != kV) {
+      f32x2 v[2][4], y[2][4], ss2 = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float m0 = kv4::bf_lo(x[k]) * inv * kv4::bf_lo(wm[k]), m1 = kv4::bf_hi(x[k]) * inv * kv4::bf_hi(wm[k]);
-      const float p0 = kv4::bf_lo(xp[k]) * inv * kv4::bf_lo(wp[k]), p1 = kv4::bf_hi(xp[k]) * inv * kv4::bf_hi(wp[k]);
-      x[k] = kv4::pack2(m0 * c[2 * k] + p0 * s[2 * k], m1 * c[2 * k + 1] + p1 * s[2 * k + 1]);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[i][k] = kv4::widen(x[i][k]);
+          ss2 = kv4::fma2(v[i][k], v[i][k], ss2);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f32x2 p;
+          if constexpr (FULL) {
+            p = v[1 - i][k];
+          } else {  // the unit lies in lane other % L, as its first or its second
+            const uint32_t a = __shfl_sync(0xffffffffu, x[0][k], other[i] % L, L);
+            const uint32_t b = __shfl_sync(0xffffffffu, x[1][k], other[i] % L, L);
+            p = kv4::widen(other[i] < L ? a : b);
+          }
+          y[i][k] = kv4::fma2(v[i][k], cw[i][k], kv4::mul2(p, sw[i][k]));
+        }
+      if (w != nullptr) {
+        float ss, hi;
+        kv4::split2(ss2, ss, hi);
+        ss += hi;
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(fmaf(ss, 1.f / HD, P.eps));
+        const f32x2 inv2 = kv4::make2(inv, inv);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[i][k] = kv4::mul2(y[i][k], inv2);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] = kv4::narrow(y[i][k]);
+      __nv_bfloat16* dst = nullptr;
+      if (P.q_out == nullptr)
+        dst = src + static_cast<int64_t>(h) * HD;
+      else if (KIND == kQ)
+        dst = P.q_out + (t * P.hq + h) * HD + 8 * l;
+      else if (P.k_out != nullptr)
+        dst = P.k_out + (t * P.hkv + h) * HD + 8 * l;
+      if (dst != nullptr && h < rows) {
+        *reinterpret_cast<int4*>(dst) = make_int4(x[0][0], x[0][1], x[0][2], x[0][3]);
+        *reinterpret_cast<int4*>(dst + HD / 2) = make_int4(x[1][0], x[1][1], x[1][2], x[1][3]);
+      }
     }
-    const int4 y = make_int4(x[0], x[1], x[2], x[3]);
-    if (P.q_out == nullptr)
-      *reinterpret_cast<int4*>(row) = y;
-    else if (is_q)
-      *reinterpret_cast<int4*>(P.q_out + (t * P.hq + h) * HD + 8 * l) = y;
-    else if (P.k_out != nullptr)
-      *reinterpret_cast<int4*>(P.k_out + (t * P.hkv + h - P.hq) * HD + 8 * l) = y;
-  }
-  const int64_t slot = ok ? P.slots[t] : -1;
-  const bool store = !is_q && slot >= 0 && slot < static_cast<int64_t>(P.cache.num_blocks) * P.cache.page;
-  uint8_t* dst = nullptr;
-  if (store) {
-    const int64_t blk = slot / P.cache.page, off = slot - blk * P.cache.page;
-    dst = P.cache.base + blk * P.cache.block_stride + (is_v ? P.cache.outer_stride : 0) + off * P.cache.token_stride +
-          static_cast<int64_t>(h - P.hq - (is_v ? P.hkv : 0)) * P.cache.head_stride;
-  }
-  if constexpr (KV4) {
-    uint32_t scale_zero;
-    const uint32_t codes = kv4::quantise8(x, &scale_zero);
-    if (store) {
-      kv4::store_codes<HD>(dst, l, is_v, codes);
-      if ((l & 3) == 0) reinterpret_cast<uint32_t*>(dst + HD / 2)[l >> 2] = scale_zero;
-      constexpr int kUsed = HD / 2 + HD / 8;
-      if constexpr (kUsed < kv4::row_bytes(HD))
-        if (l < (kv4::row_bytes(HD) - kUsed) / 4) reinterpret_cast<uint32_t*>(dst + kUsed)[l] = 0u;
+    if constexpr (KIND != kQ) {
+      if (cache_row != nullptr) {  // the whole warp's: one token
+        uint8_t* dst = cache_row + (KIND == kV ? P.cache.outer_stride : 0) + h * P.cache.head_stride;
+        if constexpr (KV4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t scale_zero;
+            const uint32_t codes = kv4::quantise8(x[i], &scale_zero);
+            if (h < rows) {
+              kv4::store_codes<HD>(dst, l + i * L, KIND == kV, codes);
+              if ((l & 3) == 0) reinterpret_cast<uint32_t*>(dst + HD / 2)[(l + i * L) >> 2] = scale_zero;
+            }
+          }
+          constexpr int kUsed = HD / 2 + HD / 8;
+          if constexpr (kUsed < kv4::row_bytes(HD))
+            if (h < rows && l < (kv4::row_bytes(HD) - kUsed) / 4) reinterpret_cast<uint32_t*>(dst + kUsed)[l] = 0u;
+        } else if (h < rows) {
+          reinterpret_cast<int4*>(dst)[l] = make_int4(x[0][0], x[0][1], x[0][2], x[0][3]);
+          reinterpret_cast<int4*>(dst)[l + L] = make_int4(x[1][0], x[1][1], x[1][2], x[1][3]);
+        }
+      }
     }
-  } else if (store) {
-    reinterpret_cast<int4*>(dst)[l] = make_int4(x[0], x[1], x[2], x[3]);
   }
+}
+
+template <int HD, bool KV4, bool FULL>
+__global__ void __launch_bounds__(kThreads, 3) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (item >= P.tokens * P.items_div.d) return;
+  const int64_t t = P.items_div.div(static_cast<uint32_t>(item));
+  const int begin = static_cast<int>(item - t * P.items_div.d) * P.steps_item;
+  const int end = begin + P.steps_item;
+  const int32_t pos = P.positions[t];
+  if (pos < 0 || pos >= P.max_pos) return;  // a token outside the table is left alone
+  uint8_t* cache_row = nullptr;
+  if (end > P.steps_q) cache_row = P.cache.row(P.slots[t]);
+
+  const int k0 = P.steps_q, v0 = k0 + P.steps_kv;
+  if (begin < k0) write_rows<HD, KV4, FULL, kQ>(P, t, begin, min(end, k0), pos, nullptr);
+  if (begin < v0 && end > k0) write_rows<HD, KV4, FULL, kK>(P, t, max(begin, k0) - k0, min(end, v0) - k0, pos, cache_row);
+  if (end > v0) write_rows<HD, KV4, FULL, kV>(P, t, max(begin, v0) - v0, min(end - v0, P.steps_kv), pos, cache_row);
 }
 
 // ---------------------------------------------------------------------------
 // Rows of the cache back to bf16: k_out[t][h] / v_out[t][h] = z + s c of slot
-// slots[t] (zeros for a slot outside the pool).
+// slots[t] (zeros for a slot outside the pool). HBM bounds it, 5 bits an element
+// in and 16 out: lanes hold rows as in the write, and a warp has kReadFly steps of
+// 512 / HD rows in flight.
 // ---------------------------------------------------------------------------
+constexpr int kReadFly = 2;
 struct GatherParams {
   Cache cache;
   const int64_t* slots;
   int64_t tokens;
+  FastDiv items_div;  // divides by the items of a token: groups of kReadFly steps of its K rows, then of its V rows
   __nv_bfloat16* k_out;
   __nv_bfloat16* v_out;
 };
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const __grid_constant__ GatherParams P) {
-  constexpr int L = HD / 8;
-  const int l = threadIdx.x % L;
-  const int64_t item = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / L;
-  const int64_t t = item / (2 * P.cache.heads);
-  if (t >= P.tokens) return;
-  const int r = static_cast<int>(item - t * 2 * P.cache.heads);
-  const bool value = r >= P.cache.heads;
-  const int h = value ? r - P.cache.heads : r;
-  const int64_t slot = P.slots[t];
-  int4 o = make_int4(0, 0, 0, 0);
-  if (slot >= 0 && slot < static_cast<int64_t>(P.cache.num_blocks) * P.cache.page) {
-    const int64_t blk = slot / P.cache.page, off = slot - blk * P.cache.page;
-    const uint8_t* row = P.cache.base + blk * P.cache.block_stride + (value ? P.cache.outer_stride : 0) +
-                         off * P.cache.token_stride + static_cast<int64_t>(h) * P.cache.head_stride;
-    o = kv4::dequantise8(kv4::load_codes<HD>(row, l, value), reinterpret_cast<const uint32_t*>(row + HD / 2)[l >> 2]);
+  constexpr int L = HD / 16, R = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane % L, r = lane / L;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  if (item >= P.tokens * P.items_div.d) return;
+  const int64_t t = P.items_div.div(static_cast<uint32_t>(item));
+  int group = static_cast<int>(item - t * P.items_div.d);
+  const bool value = group >= static_cast<int>(P.items_div.d / 2);
+  if (value) group -= P.items_div.d / 2;
+  const uint8_t* row = P.cache.row(P.slots[t]);
+  __nv_bfloat16* out = (value ? P.v_out : P.k_out) + t * P.cache.heads * HD;
+  uint32_t codes[kReadFly][2], par[kReadFly][2];
+#pragma unroll
+  for (int u = 0; u < kReadFly; ++u) {
+    const int h = (group * kReadFly + u) * R + r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) codes[u][i] = par[u][i] = 0u;
+    if (row != nullptr && h < P.cache.heads) {
+      const uint8_t* src = row + (value ? P.cache.outer_stride : 0) + h * P.cache.head_stride;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        codes[u][i] = kv4::load_codes<HD>(src, l + i * L, value);
+        par[u][i] = reinterpret_cast<const uint32_t*>(src + HD / 2)[(l + i * L) >> 2];
+      }
+    }
   }
-  reinterpret_cast<int4*>((value ? P.v_out : P.k_out) + (t * P.cache.heads + h) * HD)[l] = o;
+#pragma unroll
+  for (int u = 0; u < kReadFly; ++u) {
+    const int h = (group * kReadFly + u) * R + r;
+    if (h < P.cache.heads) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<int4*>(out + h * HD)[l + i * L] = kv4::dequantise8(codes[u][i], par[u][i]);
+    }
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -185,7 +292,8 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
                                           void* q_out, void* k_out, cudaStream_t stream) {
   if (tokens == 0) return cudaSuccess;
   WriteParams P{};
-  P.cache = Cache{static_cast<uint8_t*>(kv), block_stride, outer_stride, token_stride, head_stride, page, num_blocks, hkv};
+  P.cache = Cache{static_cast<uint8_t*>(kv), block_stride, outer_stride, token_stride, head_stride, page, num_blocks, hkv,
+                  FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (tokens < 0 || hq < 0 || !cache_ok(P.cache) || !qkv || !positions || !cos_sin || !slots || !aligned16(qkv) ||
       qkv_stride % 8 != 0 || !aligned16(cos_sin) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(q_weight) ||
       !aligned16(k_weight) || rot <= 0 || rot > hd || rot % 16 != 0 || max_pos < 0 || (bits != 4 && bits != 16) ||
@@ -206,15 +314,28 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   P.slots = slots;
   P.q_out = static_cast<__nv_bfloat16*>(q_out);
   P.k_out = static_cast<__nv_bfloat16*>(k_out);
-  const int64_t ctas = (tokens * (hq + 2 * hkv) * (hd / 8) + kThreads - 1) / kThreads;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(ctas);
+  if (hd != 64 && hd != 128 && hd != 256) return cudaErrorInvalidValue;
+  const int rows_step = 512 / hd;
+  P.steps_q = (hq + rows_step - 1) / rows_step;
+  P.steps_kv = (hkv + rows_step - 1) / rows_step;
+  // a whole token a warp when there are warps enough to fill the GPU's 148 x 32 places; else its rows are spread
+  const int steps = P.steps_q + 2 * P.steps_kv;
+  const int64_t items = std::min<int64_t>(steps, std::max<int64_t>(1, (2 * 148 * 32 + tokens - 1) / tokens));
+  P.steps_item = static_cast<int>((steps + items - 1) / items);
+  P.items_div = FastDiv(static_cast<uint32_t>((steps + P.steps_item - 1) / P.steps_item));
+  const int64_t warps = tokens * P.items_div.d;
+  if (warps > 0x7fffffff) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32));
 #define KVBM_WRITE(HD)                                                                           \
   case HD:                                                                                       \
-    if (bits == 4)                                                                               \
-      qk_norm_rope_kv_write_kernel<HD, true><<<grid, kThreads, 0, stream>>>(P);                  \
+    if (bits == 4 && rot == HD)                                                                  \
+      qk_norm_rope_kv_write_kernel<HD, true, true><<<grid, kThreads, 0, stream>>>(P);            \
+    else if (bits == 4)                                                                          \
+      qk_norm_rope_kv_write_kernel<HD, true, false><<<grid, kThreads, 0, stream>>>(P);           \
+    else if (rot == HD)                                                                          \
+      qk_norm_rope_kv_write_kernel<HD, false, true><<<grid, kThreads, 0, stream>>>(P);           \
     else                                                                                         \
-      qk_norm_rope_kv_write_kernel<HD, false><<<grid, kThreads, 0, stream>>>(P);                 \
+      qk_norm_rope_kv_write_kernel<HD, false, false><<<grid, kThreads, 0, stream>>>(P);          \
     break;
   switch (hd) {
     KVBM_WRITE(64)
@@ -232,16 +353,19 @@ extern "C" int kvbm_kv4_gather(const void* kv, int64_t block_stride, int64_t out
   if (tokens == 0) return cudaSuccess;
   GatherParams P{};
   P.cache = Cache{static_cast<uint8_t*>(const_cast<void*>(kv)), block_stride, outer_stride, token_stride, head_stride,
-                  page, num_blocks, heads};
+                  page, num_blocks, heads, FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (tokens < 0 || !cache_ok(P.cache) || !slots || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
     return cudaErrorInvalidValue;
   P.slots = slots;
   P.tokens = tokens;
   P.k_out = static_cast<__nv_bfloat16*>(k_out);
   P.v_out = static_cast<__nv_bfloat16*>(v_out);
-  const int64_t ctas = (tokens * 2 * heads * (hd / 8) + kThreads - 1) / kThreads;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(ctas);
+  if (hd != 64 && hd != 128 && hd != 256) return cudaErrorInvalidValue;
+  const int steps = (heads * (hd / 16) + 31) / 32;  // of a token's K (V) rows
+  P.items_div = FastDiv(2 * static_cast<uint32_t>((steps + kReadFly - 1) / kReadFly));
+  const int64_t warps = tokens * P.items_div.d;
+  if (warps > 0x7fffffff) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32));
   switch (hd) {
     case 64: kv4_gather_kernel<64><<<grid, kThreads, 0, stream>>>(P); break;
     case 128: kv4_gather_kernel<128><<<grid, kThreads, 0, stream>>>(P); break;
@@ -273,7 +397,7 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
   if (batch == 0) return cudaSuccess;
   kv4::AttnParams P{};
   P.cache = Cache{static_cast<uint8_t*>(const_cast<void*>(kv)), block_stride, outer_stride, token_stride, head_stride,
-                  page, num_blocks, hkv};
+                  page, num_blocks, hkv, FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (batch < 0 || batch > 65535 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || !cache_ok(P.cache) || !q || !aligned16(q) ||
       q_stride % 8 != 0 || !out || !aligned16(out) || !seq_lens || max_blocks < 0 || (max_blocks > 0 && !block_table) ||
       ctas < 0 || sm_count <= 0 || !scratch || !aligned16(scratch))
@@ -300,7 +424,6 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
   P.part_ml = scratch + rows * hd;
   P.first = reinterpret_cast<int64_t*>(scratch + rows * (hd + 2));
   P.out = static_cast<__nv_bfloat16*>(out);
-  P.page_div = FastDiv(static_cast<uint32_t>(page));
   return kv4::launch_decode(P, hd, plan, stream);
 }
 

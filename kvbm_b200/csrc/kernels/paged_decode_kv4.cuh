@@ -77,7 +77,6 @@ struct AttnParams {
   float* part_ml;   // [cta][2][hq][2]
   int64_t* first;   // [batch] first round of a request, then the rounds a CTA takes; for the merge kernel
   __nv_bfloat16* out;
-  FastDiv page_div;
 };
 
 constexpr int kHeads = 8;       // query heads a warp takes at most
@@ -377,8 +376,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           const int t = t_begin + (tile + (lane >> 1)) * round_tokens + (lane & 1) * kUnit;
           id = -1;
           if (tile + (lane >> 1) < mine && t < seq) {
-            const uint32_t col = P.page_div.div(static_cast<uint32_t>(t));
-            at = P.page_div.mod(static_cast<uint32_t>(t), col);
+            const uint32_t col = P.cache.page_div.div(static_cast<uint32_t>(t));
+            at = P.cache.page_div.mod(static_cast<uint32_t>(t), col);
             id = table[col];
             if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(P.cache.num_blocks)) id = -1;
           }
@@ -396,8 +395,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       } else {  // every row looks its own page up
         int32_t row_block = -1, row_at = 0;
         if (t0 + lane < seq) {
-          const uint32_t col = P.page_div.div(static_cast<uint32_t>(t0 + lane));
-          row_at = P.page_div.mod(static_cast<uint32_t>(t0 + lane), col);
+          const uint32_t col = P.cache.page_div.div(static_cast<uint32_t>(t0 + lane));
+          row_at = P.cache.page_div.mod(static_cast<uint32_t>(t0 + lane), col);
           row_block = table[col];
           if (static_cast<uint32_t>(row_block) >= static_cast<uint32_t>(P.cache.num_blocks)) row_block = -1;
         }

@@ -10,6 +10,8 @@ import ctypes as C
 import threading
 from pathlib import Path
 
+import torch
+
 from .. import _build
 
 MAX_LAYERS = 128
@@ -251,36 +253,30 @@ class on_device:
     """Makes ``device`` current and, given a stream (``torch.cuda.Stream`` or handle), that stream: what is
     allocated inside belongs to the stream the kernel runs on. Yields the stream's handle."""
 
-    __slots__ = ("_dev", "_stream", "_prev", "_ctx")
+    __slots__ = ("_idx", "_stream", "_prev", "_ctx")
 
-    def __init__(self, device, stream=None):
-        import torch
-
+    def __init__(self, device: torch.device, stream=None):
         if device.type != "cuda":
             raise ValueError(f"the kernels take CUDA tensors, not tensors on {device}")
-        if stream is not None and not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=device)
-        if stream is not None and stream.device != device:
-            raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        self._dev, self._stream, self._ctx, self._prev = device, stream, None, -1
+        if stream is not None:
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(int(stream), device=device)
+            if stream.device != device:
+                raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        self._idx, self._stream, self._ctx, self._prev = device.index, stream, None, -1
 
     def __enter__(self) -> int:
-        import torch
-
-        cur = torch.cuda.current_device()
-        if self._dev.index != cur:
+        cur = torch._C._cuda_getDevice()
+        if self._idx != cur:
             self._prev = cur
-            torch.cuda.set_device(self._dev.index)
-        s = self._stream
-        if s is None:
-            return torch.cuda.current_stream().cuda_stream
-        self._ctx = torch.cuda.stream(s)
+            torch.cuda.set_device(self._idx)
+        if self._stream is None:
+            return torch._C._cuda_getCurrentRawStream(self._idx)
+        self._ctx = torch.cuda.stream(self._stream)
         self._ctx.__enter__()
-        return s.cuda_stream
+        return self._stream.cuda_stream
 
     def __exit__(self, *exc) -> None:
-        import torch
-
         if self._ctx is not None:
             self._ctx.__exit__(*exc)
         if self._prev >= 0:

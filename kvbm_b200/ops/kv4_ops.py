@@ -192,7 +192,7 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
         raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} on {dev}")
     with _lib.on_device(dev, stream) as st:
         if out is None:
-            out = torch.empty(B, hq, hd, dtype=q.dtype, device=dev)
+            out = q.new_empty((B, hq, hd))
         if B == 0:
             return out
         need, sms = _decode_plan(B, hq, hkv, hd, max_blocks * kv.shape[2], ctas, dev.index)

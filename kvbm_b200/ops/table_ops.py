@@ -75,11 +75,10 @@ def batch_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_ids
             raise ValueError(f"the table has {table.shape[0]} rows for {B} requests")
     with _lib.on_device(dev, stream) as st:
         if table is None:
-            table = torch.empty(B, max_blocks, dtype=torch.int32, device=dev)
-        seq_lens = torch.empty(B, dtype=torch.int32, device=dev)
-        cu_query = torch.empty(B + 1, dtype=torch.int32, device=dev)
-        positions = torch.empty(num_tokens, dtype=torch.int32, device=dev)
-        slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+            table = query_lens.new_empty((B, max_blocks))
+        seq_lens, cu_query, positions = query_lens.new_empty(2 * B + 1 + num_tokens).split_with_sizes(
+            (B, B + 1, num_tokens))
+        slots = query_lens.new_empty(num_tokens, dtype=torch.int64)
         _lib.call("kvbm_batch_tables", query_lens.data_ptr(), context_lens.data_ptr(),
                   block_counts.data_ptr() if block_counts is not None else None, block_ids.data_ptr(),
                   block_ids.numel(), B, page, max_blocks, pad_block, table.data_ptr() or None, table.stride(0),
@@ -112,7 +111,7 @@ def slot_map(block_table: torch.Tensor, positions: torch.Tensor, *, page: int, o
         _check(out, "out", torch.int64, T, dev)
     with _lib.on_device(dev, stream) as st:
         if out is None:
-            out = torch.empty(T, dtype=torch.int64, device=dev)
+            out = positions.new_empty(T, dtype=torch.int64)
         _lib.call("kvbm_slot_map", block_table.data_ptr() or None, 0 if one else block_table.stride(0),
                   block_table.shape[1], positions.data_ptr(), T, page, out.data_ptr(), st)
     return out

@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     const int t_begin = r0 * round_tokens + stream * kTile;  // tile i begins at t_begin + i round_tokens
     const int32_t* table = P.table + b * P.table_stride;
 
-    // Starts the copies of a tile's two units; returns a bit for each of its tokens that counts.
+    // Starts the copies of a tile. TMA: returns a bit for each of its two units that is there; by rows: one for
+    // each of its tokens.
     int32_t id = -1, at = 0;    // block of the unit that this lane looked up and its first token there
     uint32_t there = 0u;        // which of the 32 units have a block
     auto issue = [&](int tile) {
@@ -370,7 +371,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       }
       const int t0 = t_begin + tile * round_tokens;
       const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
-      uint32_t live;
       if constexpr (TMA) {
         if ((tile & 15) == 0) {  // the next 32 units, one a lane
           const int t = t_begin + (tile + (lane >> 1)) * round_tokens + (lane & 1) * kUnit;
@@ -384,14 +384,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           there = __ballot_sync(0xffffffffu, id >= 0);
         }
         const uint32_t two = (there >> (2 * (tile & 15))) & 3u;
-        if (two == 0u) return 0u;
-        if ((lane >> 1) == (tile & 15)) {
+        if (two != 0u && (lane >> 1) == (tile & 15)) {
           uint64_t* bar = &full[warp][tile & 1];
           mbar_arrive_expect_tx(bar, id >= 0 ? G::kUnitBytes : 0);
           if (id >= 0) copy_unit(st + (lane & 1) * G::kUnitBytes, &map, kvh, at, id, bar);
         }
-        live = (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
-        if (seq - t0 < kTile) live &= (1u << (seq - t0)) - 1u;
+        return two;
       } else {  // every row looks its own page up
         int32_t row_block = -1, row_at = 0;
         if (t0 + lane < seq) {
@@ -400,7 +398,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           row_block = table[col];
           if (static_cast<uint32_t>(row_block) >= static_cast<uint32_t>(P.cache.num_blocks)) row_block = -1;
         }
-        live = __ballot_sync(0xffffffffu, row_block >= 0);
+        const uint32_t live = __ballot_sync(0xffffffffu, row_block >= 0);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -415,10 +413,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
                          off * P.cache.token_stride + kvh * P.cache.head_stride + piece * 16);
           }
         copy_commit();
+        return live;
       }
-      return live;
     };
-    uint32_t live_next = issue(0);
+    uint32_t next = issue(0);
 
     // ---- q as operands: column gid is head gid / 2, odd columns empty (PAIR), or head gid
     uint32_t bq[NG][2][2], bz[NZ][2];
@@ -449,8 +447,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         flag |= __shfl_xor_sync(0xffffffffu, flag, o);
       }
       const int e = max(exponent(top), -100);  // the largest element comes to [2^14, 2^15)
-      const float up = flag ? 0.f : pow2(14 - e);
-      const float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(P.qscale, 24 + e - 14);
+      const float up = flag ? 0.f : copysignf(pow2(14 - e), P.qscale);  // a negative scale turns q: factor is positive
+      float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(P.qscale), 24 + e - 14);
+      if (fac < 1e-36f) fac = 1e-36f;  // (times -infinity is to be -infinity)
       float qs[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -486,7 +485,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       for (int n = 0; n < NH; ++n) factor[n] = __shfl_sync(0xffffffffu, fac, 8 * tig + 4 * n);
     }
 
-    // ---- running state: of query head tig (PAIR) or 2 tig + n
+    // ---- running state: of query head tig (PAIR) or 2 tig + n; m in the scores' unit before factor
     float m[NH], l[NH], z[NH][NG];
     float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24 (16 f 2^-24 for odd i)
     float vf = pow2(100);  // f; the first tile sets it
@@ -503,29 +502,45 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     }
 
     for (int tile = 0; tile < mine; ++tile) {
-      const uint32_t live = live_next;
-      live_next = issue(tile + 1);
+      const uint32_t here = next;
+      next = issue(tile + 1);
       if constexpr (!TMA) {
         copy_wait<1>();
         __syncwarp();
       }
-      if (live == 0u) continue;
+      if (here == 0u) continue;
       if constexpr (TMA) {
         const int k = tile & 1;
-        if (!mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs)) given_up = true;
-        if (__any_sync(0xffffffffu, given_up)) {  // leave, when both copies in flight have ended or are given up
-          given_up = true;
-          report_status(&g_kv4_status, kStatusPipelineTimeout);
-          mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
-          if (live_next != 0u) mbar_wait_bounded(&full[warp][k ^ 1], (phases >> (k ^ 1)) & 1u, kWaitNs);
+        bool ok = mbar_try_wait(&full[warp][k], (phases >> k) & 1u);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
+          if (!__all_sync(0xffffffffu, ok)) {  // leave, when both copies in flight have ended or are given up
+            given_up = true;
+            report_status(&g_kv4_status, kStatusPipelineTimeout);
+            mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
+            if (next != 0u) mbar_wait_bounded(&full[warp][k ^ 1], (phases >> (k ^ 1)) & 1u, kWaitNs);
 #pragma unroll
-          for (int n = 0; n < NH; ++n) l[n] = __uint_as_float(0x7fc00000u);
-          break;
+            for (int n = 0; n < NH; ++n) l[n] = __uint_as_float(0x7fc00000u);
+            break;
+          }
         }
         phases ^= 1u << k;
       }
       const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
-      const bool whole = live == 0xffffffffu;
+      const int left = seq - (t_begin + tile * round_tokens);  // tokens from this tile's first on, at least 1
+      const bool whole = here == (TMA ? 3u : 0xffffffffu) && left >= kTile;
+      uint32_t live = 0xffffffffu;
+      if (!whole) {  // a bit for each token that counts; V of the others, which may hold anything, becomes zeros
+        live = TMA ? (here & 1u ? 0xffffu : 0u) | (here & 2u ? 0xffff0000u : 0u) : here;
+        if (left < kTile) live &= (1u << left) - 1u;
+        if (!((live >> lane) & 1u)) {
+          const uint32_t par = st + (lane >> 4) * G::kUnitBytes + (kUnit + (lane & 15)) * G::kRow + HD / 2;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) asm volatile("st.shared.b32 [%0], %1;" ::"r"(par + 4 * g), "r"(0) : "memory");
+        }
+        if constexpr (TMA) fence_proxy_async_smem();  // the next copy into this place comes behind
+        __syncwarp();
+      }
 
       // ---- scores of tokens gid, gid + 8 of both units
       float s[2][2][NH];
@@ -568,10 +583,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       float alpha[NH];
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) s[u][r][n] *= factor[n];
         if (!whole) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -583,8 +594,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         top = fmaxf(m[n], top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        alpha[n] = ex2(m[n] - ref);
+        const float ref = top == -INFINITY ? 0.f : top * factor[n];
+        alpha[n] = ex2(fmaf(m[n], factor[n], -ref));
         m[n] = top;
         l[n] *= alpha[n];
 #pragma unroll
@@ -593,7 +604,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            s[u][r][n] = ex2(s[u][r][n] - ref);
+            s[u][r][n] = ex2(fmaf(s[u][r][n], factor[n], -ref));
             l[n] += s[u][r][n];
           }
       }
@@ -605,10 +616,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           lds(par[u][r], st + u * G::kUnitBytes + (kUnit + gid + 8 * r) * G::kRow + HD / 2);
-          if (!whole && !((live >> (16 * u + 8 * r + gid)) & 1u)) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) par[u][r][g] = 0u;  // what lies behind the last token may be a NaN
-          }
 #pragma unroll
           for (int g = 0; g < NG; ++g) top = fmaxf(top, bf_lo(par[u][r][g]));
         }
@@ -696,6 +703,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     if constexpr (!TMA) copy_wait<0>();
     __syncwarp();
 
+#pragma unroll
+    for (int n = 0; n < NH; ++n) m[n] = m[n] == -INFINITY ? m[n] : m[n] * factor[n];
     // ---- sums over the lanes that share a head; codes' unit and f out of the sums, zeros' part in
 #pragma unroll
     for (int n = 0; n < NH; ++n) {

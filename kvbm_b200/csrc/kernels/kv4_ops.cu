@@ -382,7 +382,7 @@ extern "C" int kvbm_paged_decode_attn_kv4_plan(int batch, int hq, int hkv, int h
   if (!out || batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || max_tokens < 0 || ctas < 0 || sm_count <= 0)
     return cudaErrorInvalidValue;
   const kv4::Plan p = kv4::plan_decode(batch, hq, hkv, hd, max_tokens, ctas, sm_count);
-  out[0] = static_cast<int64_t>(p.ctas) * 2 * hq * (hd + 2) + 2 * (static_cast<int64_t>(batch) + 1);
+  out[0] = static_cast<int64_t>(p.ctas) * 2 * hq * (hd + 2) + 2 * static_cast<int64_t>(batch);
   out[1] = p.ctas;
   return cudaSuccess;
 }
@@ -422,7 +422,7 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
   const int64_t rows = static_cast<int64_t>(plan.ctas) * 2 * hq;
   P.part_acc = scratch;
   P.part_ml = scratch + rows * hd;
-  P.first = reinterpret_cast<int64_t*>(scratch + rows * (hd + 2));
+  P.parts = reinterpret_cast<int2*>(scratch + rows * (hd + 2));
   P.out = static_cast<__nv_bfloat16*>(out);
   return kv4::launch_decode(P, hd, plan, stream);
 }

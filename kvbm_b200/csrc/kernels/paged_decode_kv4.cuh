@@ -14,25 +14,28 @@
 // dequantised:
 //
 // A nibble masked in place is a subnormal fp16: c 2^-24 in bits 0-3, c 2^-20 in
-// bits 4-7, both exact. So a word of 8 codes becomes 4 operand registers with
-// one shift and four ands, and the factor 16 goes to the other operand (scores)
-// or to the end (P V).
+// bits 4-7, both exact, and so is a whole byte, (c0 + 16 c1) 2^-24. A word of 8
+// codes becomes 4 operand registers, c0 and c0 + 16 c1 of its even and of its odd
+// bytes, with three ands and one byte permute; what multiplies or follows them
+// takes the two apart: a c0 + b c1 = (a - b / 16) c0 + (b / 16) (c0 + 16 c1).
 //
-// Scores. q 2^k in fp16 is exact (bf16 has 8 bits; k puts the head's largest
-// element at 2^14, elements below 2^-28 of it lose bits). Each group of 32 is two
-// m16n8k16 products, whose fp32 sums take the group's scale; the zeros' part,
+// Scores. q 2^k is put in fp16, k bringing the head's largest element to 2^13.
+// (a - b / 16) of two q needs more bits than fp16 has: with up to 4 query heads on
+// a KV head (PAIR) it goes in two parts, in two of the 8 columns of a product, and
+// 2^-22 of it is lost at most; with 5 to 8 there are no columns to spare, and c1 is
+// taken alone at one shift more a word. Each group of 32 is two m16n8k16 products, whose fp32 sums take the group's scale; the zeros' part,
 // sum over g of z_g (sum of q_g), is one bf16 product more with the sums of q in
 // three bf16 parts.
 //
 // P V. Codes of two tokens are paired by one byte permute. The V scale goes into
-// the weight: p' = fp16(p s f), off by at most 2^-11 of it, with f a power of
-// two that keeps the warp's largest s f in [2^13, 2^15]; f changes, and the sums
-// with it, when a larger scale comes by. Then sum p v = sum p' c / f + sum p z.
+// the weight: p' = fp16(p s f), off by at most 2^-11 of it, with f a power of two
+// that put the largest s f at [2^8, 2^9) when it was set; when sums of p' come out
+// infinite f is set again, and the sums of products with it. Then
+// sum p v = sum p' c / f + sum p z.
 // Products of 32 tokens are folded into fp32 accumulators, since the tensor
 // core's own accumulation truncates.
 //
-// With up to 4 query heads on a KV head (PAIR) the 8 columns of a P V product
-// hold p' of 4 heads for two groups: tile rows 0-7 are elements of the even
+// In PAIR the 8 columns of a P V product hold p' of 4 heads for two groups: tile rows 0-7 are elements of the even
 // group, rows 8-15 of the odd one, half of the outputs have no meaning. With 5
 // to 8 heads a column is a head and a tile lies in one group.
 //
@@ -75,7 +78,7 @@ struct AttnParams {
   float qscale;
   float* part_acc;  // [cta][2][hq][HD]
   float* part_ml;   // [cta][2][hq][2]
-  int64_t* first;   // [batch] first round of a request, then the rounds a CTA takes; for the merge kernel
+  int2* parts;      // [batch]: a request's first slot of partial results (2 cta, + 1: not its CTA's first), and how many
   __nv_bfloat16* out;
 };
 
@@ -147,9 +150,25 @@ __device__ __forceinline__ uint32_t half2(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-// Nibbles i and i + 4 of x as an fp16 pair, times 2^-24 (i even) or 2^-20 (i odd).
-__device__ __forceinline__ uint32_t code_pair(uint32_t x, int i) {
-  return (i < 2 ? x : x >> 8) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+// A word's nibbles i and i + 4 as fp16 pairs in units of 2^-24: i even c_i; i odd c_{i-1} + 16 c_i.
+__device__ __forceinline__ void code_pairs(uint32_t (&a)[4], uint32_t x) {
+  a[1] = x & 0x00ff00ffu;
+  a[0] = x & 0x000f000fu;
+  a[3] = __byte_perm(x, 0, 0x4341);
+  a[2] = a[3] & 0x000f000fu;
+}
+// The same with i odd 16 c_i alone.
+__device__ __forceinline__ void code_pairs_alone(uint32_t (&a)[4], uint32_t x) {
+  a[0] = x & 0x000f000fu;
+  a[1] = x & 0x00f000f0u;
+  x >>= 8;
+  a[2] = x & 0x000f000fu;
+  a[3] = x & 0x00f000f0u;
+}
+__device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ __forceinline__ int exponent(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127; }
@@ -165,8 +184,8 @@ __device__ __forceinline__ int rounds_of(int tokens, int streams) {
 // Merges the partial results of each request that several CTAs worked on. Part i of a request that begins in
 // CTA c lies in CTA c + i, in the slot of that CTA's first request (0), or of a later one (1: only its last can go
 // on). A warp reads 32 parts' (m, l), a lane each, and up to 16 parts' acc at a time, lane l elements l E ..
-// (E = HD / 32). A CTA takes `heads_cta` query heads of a request: few parts are merged by one warp a head, many by
-// all warps, head by head.
+// (E = HD / 32). A CTA takes 8 query heads of a request: few parts are merged by one warp a head, many by all
+// warps, head by head.
 constexpr int kMergeWarps = 8;
 template <int HD>
 __device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, int64_t slot0, int begin, int step, int n,
@@ -215,23 +234,20 @@ __device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, i
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __grid_constant__ AttnParams P,
-                                                                     int heads_cta) {
+__global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __grid_constant__ AttnParams P) {
   constexpr int E = HD / 32;
   __shared__ float red[kMergeWarps][HD + 2];
-  const int b = blockIdx.y, h_begin = blockIdx.x * heads_cta, h_end = min(P.hq, h_begin + heads_cta);
+  const int b = blockIdx.y, h_begin = blockIdx.x * kMergeWarps, h_end = min(P.hq, h_begin + kMergeWarps);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rounds = rounds_of(tokens_of(P, b), P.streams);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t first = P.first[b], per = P.first[P.batch];
-  const int64_t c0 = first / per;
-  const int n = static_cast<int>((first + rounds - 1) / per - c0) + 1;
+  const int2 parts = __ldcg(&P.parts[b]);
+  const int n = parts.y;
   if (n == 1) return;  // written by its one CTA
-  const int64_t slot0 = first == c0 * per ? 0 : P.hq;
-  const bool few = n <= 32;
+  const int64_t row0 = static_cast<int64_t>(parts.x & ~1) * P.hq, slot0 = (parts.x & 1) * P.hq;
+  const bool few = n <= 64;
   for (int h = h_begin + (few ? warp : 0); h < h_end; h += few ? kMergeWarps : 1) {
     float m, l, acc[E];
-    merge_parts<HD>(P, c0 * 2 * P.hq + h, slot0, few ? 0 : warp * 32, kMergeWarps * 32, n, m, l, acc);
+    merge_parts<HD>(P, row0 + h, slot0, few ? 0 : warp * 32, few ? 32 : kMergeWarps * 32, n, m, l, acc);
     if (!few) {
       __syncthreads();
 #pragma unroll
@@ -336,8 +352,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   const int64_t f_begin = f;
   int b = start_b;
   int64_t first = start_first;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) P.first[P.batch] = per;
-
   const int yw = warp % P.y_cta, stream = warp / P.y_cta;
   const int y = blockIdx.y * P.y_cta + yw;
   const bool active = y < P.y_total;
@@ -418,19 +432,19 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     };
     uint32_t next = issue(0);
 
-    // ---- q as operands: column gid is head gid / 2, odd columns empty (PAIR), or head gid
+    // ---- q as operands: column gid is head gid / 2, odd columns the second parts (PAIR), or head gid
     uint32_t bq[NG][2][2], bz[NZ][2];
     float factor[NH];
     {
       const int h = PAIR ? gid >> 1 : gid;
-      const bool mine_h = h < heads && (!PAIR || (gid & 1) == 0);
+      const bool second = PAIR && (gid & 1) != 0;
       uint32_t xw[NG][4];
       float top = 0.f;
       bool bad = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         int4 w = make_int4(0, 0, 0, 0);
-        if (mine_h)
+        if (h < heads)
           w = *reinterpret_cast<const int4*>(P.q + b * P.q_stride + (head0 + h) * static_cast<int64_t>(HD) +
                                              g * kGroup + tig * 8);
         xw[g][0] = w.x, xw[g][1] = w.y, xw[g][2] = w.z, xw[g][3] = w.w;
@@ -446,9 +460,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         flag |= __shfl_xor_sync(0xffffffffu, flag, o);
       }
-      const int e = max(exponent(top), -100);  // the largest element comes to [2^14, 2^15)
-      const float up = flag ? 0.f : copysignf(pow2(14 - e), P.qscale);  // a negative scale turns q: factor is positive
-      float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(P.qscale), 24 + e - 14);
+      const int e = max(exponent(top), -100);  // the largest element comes to [2^13, 2^14)
+      const float up = flag ? 0.f : copysignf(pow2(13 - e), P.qscale);  // a negative scale turns q: factor is positive
+      float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(P.qscale), 24 + e - 13);
       if (fac < 1e-36f) fac = 1e-36f;  // (times -infinity is to be -infinity)
       float qs[NG];
 #pragma unroll
@@ -463,11 +477,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         }
         qs[g] += __shfl_xor_sync(0xffffffffu, qs[g], 1);
         qs[g] += __shfl_xor_sync(0xffffffffu, qs[g], 2);
-        // register i of a word holds elements i and i + 4, sixteen times too large for odd i
+        // register i of a word has to do with elements i and i + 4
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          bq[g][j][0] = half2(x[2 * j], x[2 * j + 4]);
-          bq[g][j][1] = half2(0.0625f * x[2 * j + 1], 0.0625f * x[2 * j + 5]);
+          float even[2], odd[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            odd[k] = 0.0625f * x[2 * j + 1 + 4 * k];  // exact in fp16, but for the smallest elements
+            even[k] = x[2 * j + 4 * k] - (PAIR ? odd[k] : 0.f);
+            if (second) {
+              even[k] -= __half2float(__float2half_rn(even[k]));
+              odd[k] -= __half2float(__float2half_rn(odd[k]));
+            }
+          }
+          bq[g][j][0] = half2(even[0], even[1]);
+          bq[g][j][1] = half2(odd[0], odd[1]);
         }
       }
       // sums of q of group tig (+ 4) in the codes' unit 2^-24: three bf16 parts in k slots 2 tig, + 1, + 8 (the fourth: 0)
@@ -478,8 +502,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         for (int g = 4 * j; g < 4 * j + 4 && g < NG; ++g) s = (g & 3) == tig ? qs[g] : s;
         s *= pow2(-24);
         const float s1 = __bfloat162float(__float2bfloat16(s)), s2 = __bfloat162float(__float2bfloat16(s - s1));
-        bz[j][0] = pack2(s1, s2);
-        bz[j][1] = pack2(s - s1 - s2, 0.f);
+        bz[j][0] = second ? 0u : pack2(s1, s2);
+        bz[j][1] = second ? 0u : pack2(s - s1 - s2, 0.f);
       }
 #pragma unroll
       for (int n = 0; n < NH; ++n) factor[n] = __shfl_sync(0xffffffffu, fac, 8 * tig + 4 * n);
@@ -487,7 +511,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 
     // ---- running state: of query head tig (PAIR) or 2 tig + n; m in the scores' unit before factor
     float m[NH], l[NH], z[NH][NG];
-    float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24 (16 f 2^-24 for odd i)
+    float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24; odd i: that of i - 1 and 16 times i's
     float vf = pow2(100);  // f; the first tile sets it
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
@@ -569,14 +593,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           uint32_t x0[1], x1[1];
           lds(x0, k0 + g * 16 + tig * 4);
           lds(x1, k1 + g * 16 + tig * 4);
-          mma_f16(c, code_pair(x0[0], 0), code_pair(x1[0], 0), code_pair(x0[0], 1), code_pair(x1[0], 1), bq[g][0][0],
-                  bq[g][0][1], 0.f, 0.f, 0.f, 0.f);
-          mma_f16(c, code_pair(x0[0], 2), code_pair(x1[0], 2), code_pair(x0[0], 3), code_pair(x1[0], 3), bq[g][1][0],
-                  bq[g][1][1], c[0], c[1], c[2], c[3]);
+          uint32_t a0[4], a1[4];
+          if constexpr (PAIR) {
+            code_pairs(a0, x0[0]);
+            code_pairs(a1, x1[0]);
+          } else {
+            code_pairs_alone(a0, x0[0]);
+            code_pairs_alone(a1, x1[0]);
+          }
+          mma_f16(c, a0[0], a1[0], a0[1], a1[1], bq[g][0][0], bq[g][0][1], 0.f, 0.f, 0.f, 0.f);
+          mma_f16(c, a0[2], a1[2], a0[3], a1[3], bq[g][1][0], bq[g][1][1], c[0], c[1], c[2], c[3]);
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int n = 0; n < NH; ++n) s[u][r][n] = fmaf(bf_lo(par[r][g]), c[2 * r + n], s[u][r][n]);
+            for (int n = 0; n < NH; ++n)
+              s[u][r][n] = fmaf(bf_lo(par[r][g]), PAIR ? c[2 * r] + c[2 * r + 1] : c[2 * r + n], s[u][r][n]);
         }
       }
       // ---- softmax
@@ -609,22 +640,51 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           }
       }
       // ---- weights times V scales, as operands: PAIR columns are (head, group parity)
-      uint32_t par[2][2][NG];
-      float top = 0.f;
+      uint32_t par[2][2][NG], bp[2][NB][2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           lds(par[u][r], st + u * G::kUnitBytes + (kUnit + gid + 8 * r) * G::kRow + HD / 2);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) top = fmaxf(top, bf_lo(par[u][r][g]));
+          for (int n = 0; n < NH; ++n)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) z[n][g] = fmaf(s[u][r][n], bf_hi(par[u][r][g]), z[n][g]);
         }
-      if (__any_sync(0xffffffffu, top * vf > 32768.f)) {  // a larger scale than any before (the first tile's): move f
+      for (bool set = false;; set = true) {
+        uint32_t sum = 0u;  // infinite (or a NaN) if a weight is, or all are near it
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float ps[NG][NH];
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              const float pf = s[u][r][n] * vf;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) ps[g][n] = pf * bf_lo(par[u][r][g]);
+            }
+#pragma unroll
+            for (int k = 0; k < NB; ++k) {
+              const uint32_t p = PAIR ? half2(ps[2 * k][0], ps[2 * k + 1][0]) : half2(ps[k][0], ps[k][NH - 1]);
+              sum = add_half2(sum, p);
+              bp[u][k][r] = p;
+            }
+          }
+        const bool over = (sum & 0x7c00u) == 0x7c00u || (sum & 0x7c000000u) == 0x7c000000u;
+        if (set || !__any_sync(0xffffffffu, over)) break;
+        float top = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) top = fmaxf(top, bf_lo(par[u][r][g]));
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float next = pow2(max(13 - exponent(top), -126));
-        const float down = next / vf;
-        vf = next;
+        const float next_vf = fminf(vf, pow2(min(max(8 - exponent(top), -126), 100)));
+        const float down = next_vf / vf;
+        vf = next_vf;
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -632,25 +692,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[g][i][n] *= down;
       }
-      uint32_t bp[2][NB][2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float ps[NG][NH];
+        for (int k = 0; k < NB; ++k)
 #pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            const float pf = s[u][r][n] * vf;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              z[n][g] = fmaf(s[u][r][n], bf_hi(par[u][r][g]), z[n][g]);
-              ps[g][n] = pf * bf_lo(par[u][r][g]);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < NB; ++k)
-            bp[u][k][r] = transpose8x8(PAIR ? half2(ps[2 * k][0], ps[2 * k + 1][0]) : half2(ps[k][0], ps[k][NH - 1]));
-        }
+          for (int r = 0; r < 2; ++r) bp[u][k][r] = transpose8x8(bp[u][k][r]);
       // ---- acc += sum p' c: this lane's codes of tokens 2 tig, 2 tig + 1 and those 8 further
       uint32_t x[2][4][NW];
 #pragma unroll
@@ -660,22 +707,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           lds(x[u][t], st + u * G::kUnitBytes + (kUnit + 2 * tig + (t & 1) + 8 * (t >> 1)) * G::kRow + gid * NW * 4);
 #pragma unroll
       for (int k = 0; k < NW; ++k) {  // groups 2 k and 2 k + 1
-        uint32_t w[2][2][2];          // [unit][group][tokens 2 tig.. / 8 further]: codes i of the pair in nibbles i, i + 4
+        uint32_t w[2][2][2][4];       // [unit][group][tokens 2 tig.. / 8 further][register]
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            w[u][0][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x5410);
-            w[u][1][r] = __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x7632);
+            code_pairs(w[u][0][r], __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x5410));
+            code_pairs(w[u][1][r], __byte_perm(x[u][2 * r][k], x[u][2 * r + 1][k], 0x7632));
           }
         if constexpr (PAIR) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float c[4];
-            mma_f16(c, code_pair(w[0][0][0], i), code_pair(w[0][1][0], i), code_pair(w[0][0][1], i),
-                    code_pair(w[0][1][1], i), bp[0][k][0], bp[0][k][1], 0.f, 0.f, 0.f, 0.f);
-            mma_f16(c, code_pair(w[1][0][0], i), code_pair(w[1][1][0], i), code_pair(w[1][0][1], i),
-                    code_pair(w[1][1][1], i), bp[1][k][0], bp[1][k][1], c[0], c[1], c[2], c[3]);
+            mma_f16(c, w[0][0][0][i], w[0][1][0][i], w[0][0][1][i], w[0][1][1][i], bp[0][k][0], bp[0][k][1], 0.f, 0.f,
+                    0.f, 0.f);
+            mma_f16(c, w[1][0][0][i], w[1][1][0][i], w[1][0][1][i], w[1][1][1][i], bp[1][k][0], bp[1][k][1], c[0], c[1],
+                    c[2], c[3]);
             acc[2 * k][i][0] = fmaf(acc[2 * k][i][0], alpha[0], c[0]);
             acc[2 * k + 1][i][0] = fmaf(acc[2 * k + 1][i][0], alpha[0], c[3]);
           }
@@ -683,13 +730,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
           for (int p = 0; p < 2; ++p)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {  // rows 0-7: code 2 j, rows 8-15: code 2 j + 1
+            for (int j = 0; j < 2; ++j) {  // rows 0-7: register 2 j, rows 8-15: register 2 j + 1
               const int g = 2 * k + p;
               float c[4];
-              mma_f16(c, code_pair(w[0][p][0], 2 * j), code_pair(w[0][p][0], 2 * j + 1), code_pair(w[0][p][1], 2 * j),
-                      code_pair(w[0][p][1], 2 * j + 1), bp[0][g][0], bp[0][g][1], 0.f, 0.f, 0.f, 0.f);
-              mma_f16(c, code_pair(w[1][p][0], 2 * j), code_pair(w[1][p][0], 2 * j + 1), code_pair(w[1][p][1], 2 * j),
-                      code_pair(w[1][p][1], 2 * j + 1), bp[1][g][0], bp[1][g][1], c[0], c[1], c[2], c[3]);
+              mma_f16(c, w[0][p][0][2 * j], w[0][p][0][2 * j + 1], w[0][p][1][2 * j], w[0][p][1][2 * j + 1], bp[0][g][0],
+                      bp[0][g][1], 0.f, 0.f, 0.f, 0.f);
+              mma_f16(c, w[1][p][0][2 * j], w[1][p][0][2 * j + 1], w[1][p][1][2 * j], w[1][p][1][2 * j + 1], bp[1][g][0],
+                      bp[1][g][1], c[0], c[1], c[2], c[3]);
 #pragma unroll
               for (int n = 0; n < NH; ++n) {
                 acc[g][2 * j][n] = fmaf(acc[g][2 * j][n], alpha[n], c[n]);
@@ -717,8 +764,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[g][i][n] = fmaf(acc[g][i][n] * (i & 1 ? 1048576.f : 16777216.f), 1.f / vf, z[n][g]);
+        for (int i = 0; i < 4; i += 2) {
+          acc[g][i + 1][n] = fmaf((acc[g][i + 1][n] - acc[g][i][n]) * 1048576.f, 1.f / vf, z[n][g]);
+          acc[g][i][n] = fmaf(acc[g][i][n] * 16777216.f, 1.f / vf, z[n][g]);
+        }
     }
     // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
     if (P.streams > 1) {
@@ -776,7 +825,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           P.part_ml[(slot_row + h) * 2 + 1] = l[n];
         }
       }
-      if (r0 == 0 && y == 0 && lane == 0) P.first[b] = first;
+      if (r0 == 0 && y == 0 && lane == 0)
+        P.parts[b] = make_int2(2 * blockIdx.x + (f == f_begin ? 0 : 1),
+                               static_cast<int>((first + rounds - 1) / per) - static_cast<int>(blockIdx.x) + 1);
     }
     f = first + r0 + mine;
     if (r0 + mine == rounds) {
@@ -858,9 +909,7 @@ cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t
             : launch_decode_kernel<HD, false, false>(P, map, plan, stream);
   if (e != cudaSuccess || plan.ctas == 1) return e;
   cudaLaunchConfig_t cfg{};
-  // a head a CTA while that leaves SMs free for it
-  const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 1024 ? 1 : kMergeWarps;
-  cfg.gridDim = dim3((P.hq + heads_cta - 1) / heads_cta, P.batch);
+  cfg.gridDim = dim3((P.hq + kMergeWarps - 1) / kMergeWarps, P.batch);
   cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
@@ -868,7 +917,7 @@ cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD>, P, heads_cta);
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD>, P);
 }
 
 inline cudaError_t launch_decode(const AttnParams& P, int hd, const Plan& plan, cudaStream_t stream) {

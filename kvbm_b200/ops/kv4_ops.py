@@ -39,17 +39,38 @@ def _cache_args(kv: torch.Tensor, device, bits: int = 4) -> tuple:
         raise ValueError(f"the cache is on {kv.device}, expected {device}")
     if kv.dtype != (torch.uint8 if bits == 4 else torch.bfloat16):
         raise ValueError(f"a {bits}-bit cache is {torch.uint8 if bits == 4 else torch.bfloat16}, not {kv.dtype}")
-    e = kv.element_size()
     nb, _, page, heads, row = kv.shape
-    s = kv.stride()
-    if (row > 1 and s[4] != 1) or kv.data_ptr() % 16 or any(x * e % 16 for x in s[:4]):
+    block, outer, token, head, unit = kv.stride()
+    ptr = kv.data_ptr()
+    if bits == 16:
+        block, outer, token, head = 2 * block, 2 * outer, 2 * token, 2 * head
+    if (unit != 1 and row > 1) or (ptr | block | outer | token | head) & 15:
         raise ValueError("cache rows need unit stride and 16-byte aligned starts")
-    return (kv.data_ptr(), s[0] * e, s[1] * e, s[2] * e, s[3] * e, page, nb), heads, row
+    return (ptr, block, outer, token, head, page, nb), heads, row
 
 
 def _vec(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, device) -> None:
     if t.dtype != dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous {dtype} [{n}] on {device}")
+
+
+def _weight(w: torch.Tensor | None, name: str, hd: int, device) -> int | None:
+    if w is None:
+        return None
+    _vec(w, name, torch.bfloat16, hd, device)
+    ptr = w.data_ptr()
+    if ptr & 15:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    return ptr
+
+
+def _rows_out(o: torch.Tensor | None, name: str, shape: tuple, device) -> int | None:
+    if o is None:
+        return None
+    ptr = o.data_ptr()
+    if o.shape != shape or o.dtype != torch.bfloat16 or not o.is_contiguous() or o.device != device or ptr & 15:
+        raise ValueError(f"{name} must be a contiguous bf16 {list(shape)} on {device}")
+    return ptr
 
 
 def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, hq: int, hkv: int,
@@ -76,7 +97,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: t
         raise ValueError(f"qkv has {H} heads, expected {hq} + 2 * {hkv}")
     if hd not in (64, 128, 256):
         raise ValueError(f"qk_norm_rope_kv_write takes head_dim 64, 128 or 256, not {hd}")
-    if qkv.stride(2) != 1 or (H > 1 and qkv.stride(1) != hd) or (T > 1 and qkv.stride(0) % 8) or qkv.data_ptr() % 16:
+    token_stride, head_stride, unit = qkv.stride()
+    if unit != 1 or (H > 1 and head_stride != hd) or (T > 1 and token_stride & 7) or qkv.data_ptr() & 15:
         raise ValueError("qkv needs contiguous heads and 16-byte aligned tokens")
     bits = 16 if kv.dtype == torch.bfloat16 else 4
     cache, heads, row = _cache_args(kv, dev, bits)
@@ -86,28 +108,21 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: t
     _vec(positions, "positions", torch.int32, T, dev)
     _vec(slots, "slots", torch.int64, T, dev)
     if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.device != dev \
-            or cos_sin.data_ptr() % 16:
+            or cos_sin.data_ptr() & 15:
         raise ValueError("cos_sin must be a contiguous fp32 [max_position, rot] on the same device")
-    rot = cos_sin.shape[1]
+    max_pos, rot = cos_sin.shape
     if rot < 16 or rot > hd or rot % 16:
         raise ValueError(f"rot {rot} must be a multiple of 16 up to head_dim {hd}")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _vec(w, name, torch.bfloat16, hd, dev)
-            if w.data_ptr() % 16:
-                raise ValueError(f"{name} must be 16-byte aligned")
     if k_out is not None and q_out is None:
         raise ValueError("k_out needs q_out")
-    for o, name, n in ((q_out, "q_out", hq), (k_out, "k_out", hkv)):
-        if o is not None and (o.shape != (T, n, hd) or o.dtype != torch.bfloat16 or not o.is_contiguous()
-                              or o.device != dev or o.data_ptr() % 16):
-            raise ValueError(f"{name} must be a contiguous bf16 [{T}, {n}, {hd}] on {dev}")
+    qw = _weight(q_weight, "q_weight", hd, dev)
+    kw = _weight(k_weight, "k_weight", hd, dev)
+    qo = _rows_out(q_out, "q_out", (T, hq, hd), dev)
+    ko = _rows_out(k_out, "k_out", (T, hkv, hd), dev)
     with _lib.on_device(dev, stream) as st:
-        _lib.call("kvbm_qk_norm_rope_kv_write", qkv.data_ptr(), qkv.stride(0), T, hq, hkv, hd, rot,
-                  positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0],
-                  q_weight.data_ptr() if q_weight is not None else None,
-                  k_weight.data_ptr() if k_weight is not None else None, eps, bits, *cache, slots.data_ptr(),
-                  q_out.data_ptr() if q_out is not None else None, k_out.data_ptr() if k_out is not None else None, st)
+        _lib.call("kvbm_qk_norm_rope_kv_write", qkv.data_ptr(), token_stride, T, hq, hkv, hd, rot,
+                  positions.data_ptr(), cos_sin.data_ptr(), max_pos, qw, kw, eps, bits, *cache, slots.data_ptr(),
+                  qo, ko, st)
 
 
 def kv4_gather(kv: torch.Tensor, slots: torch.Tensor, *, k_out: torch.Tensor | None = None,
@@ -120,15 +135,14 @@ def kv4_gather(kv: torch.Tensor, slots: torch.Tensor, *, k_out: torch.Tensor | N
         raise ValueError(f"a 4-bit cache has rows of 48, 80 or 160 bytes, not {row}")
     T = slots.numel()
     _vec(slots, "slots", torch.int64, T, dev)
-    for o, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if o is not None and (o.shape != (T, heads, hd) or o.dtype != torch.bfloat16 or not o.is_contiguous()
-                              or o.device != dev or o.data_ptr() % 16):
-            raise ValueError(f"{name} must be a contiguous bf16 [{T}, {heads}, {hd}] on {dev}")
+    shape = (T, heads, hd)
+    _rows_out(k_out, "k_out", shape, dev)
+    _rows_out(v_out, "v_out", shape, dev)
     with _lib.on_device(dev, stream) as st:
         if k_out is None:
-            k_out = torch.empty(T, heads, hd, dtype=torch.bfloat16, device=dev)
+            k_out = kv.new_empty(shape, dtype=torch.bfloat16)
         if v_out is None:
-            v_out = torch.empty(T, heads, hd, dtype=torch.bfloat16, device=dev)
+            v_out = torch.empty_like(k_out)
         _lib.call("kvbm_kv4_gather", *cache, heads, hd, slots.data_ptr(), T, k_out.data_ptr(), v_out.data_ptr(), st)
     return k_out, v_out
 
@@ -173,7 +187,8 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
         raise ValueError(f"the cache's rows of {row} bytes do not hold head_dim {hd}")
     if hq < 1 or hq % hkv:
         raise ValueError(f"{hq} query heads are not a multiple of the cache's {hkv}")
-    if q.stride(2) != 1 or (hq > 1 and q.stride(1) != hd) or (B > 1 and q.stride(0) % 8) or q.data_ptr() % 16:
+    row_stride, head_stride, unit = q.stride()
+    if unit != 1 or (hq > 1 and head_stride != hd) or (B > 1 and row_stride & 7) or q.data_ptr() & 15:
         raise ValueError("q needs contiguous heads and 16-byte aligned rows")
     if B > 65535:
         raise ValueError(f"at most 65,535 requests, got {B}")
@@ -187,9 +202,7 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
     if scratch is not None and (scratch.dtype != torch.float32 or scratch.device != dev
                                 or not scratch.is_contiguous() or scratch.data_ptr() % 16):
         raise ValueError(f"scratch must be 16-byte aligned fp32 on {dev}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()
-                            or out.device != dev or out.data_ptr() % 16):
-        raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} on {dev}")
+    _rows_out(out, "out", (B, hq, hd), dev)
     with _lib.on_device(dev, stream) as st:
         if out is None:
             out = q.new_empty((B, hq, hd))
@@ -200,7 +213,7 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
             scratch = torch.empty(need, dtype=torch.float32, device=dev)
         elif scratch.numel() < need:
             raise ValueError(f"scratch holds {scratch.numel()} floats, {need} are needed")
-        _lib.call("kvbm_paged_decode_attn_kv4", q.data_ptr(), q.stride(0), *cache, block_table.data_ptr() or None,
+        _lib.call("kvbm_paged_decode_attn_kv4", q.data_ptr(), row_stride, *cache, block_table.data_ptr() or None,
                   block_table.stride(0), max_blocks, seq_lens.data_ptr(), B, hq, hkv, hd, softmax_scale, ctas, sms,
                   scratch.data_ptr(), out.data_ptr(), st)
     return out

@@ -177,29 +177,48 @@ __device__ __forceinline__ int tokens_of(const AttnParams& P, int b) {
   return static_cast<int>(min(static_cast<int64_t>(max(P.seq_lens[b], 0)),
                               min(static_cast<int64_t>(P.max_blocks) * P.cache.page, static_cast<int64_t>(0x7ffff000))));
 }
-// Rounds of streams x 32 tokens; an empty request has one, so that its zeros are written like any result.
+// Rounds of streams x 32 tokens that a request counts for: its own, and kStart in front of them in which nothing
+// is done, for what it costs a CTA to begin a request.
+constexpr int kStart = 2;
 __device__ __forceinline__ int rounds_of(int tokens, int streams) {
-  return max((tokens + kTile * streams - 1) / (kTile * streams), 1);
+  return kStart + (tokens + kTile * streams - 1) / (kTile * streams);
 }
 // Merges the partial results of each request that several CTAs worked on. Part i of a request that begins in
 // CTA c lies in CTA c + i, in the slot of that CTA's first request (0), or of a later one (1: only its last can go
-// on). A warp reads 32 parts' (m, l), a lane each, and up to 16 parts' acc at a time, lane l elements l E ..
-// (E = HD / 32). A CTA takes 8 query heads of a request: few parts are merged by one warp a head, many by all
-// warps, head by head.
+// on). A warp reads 32 parts' (m, l), a lane each, together with 64 / E parts' acc, of which lane l has elements
+// l E .. (E = HD / 32): the bound is the latency of that one round of loads. A CTA takes 8 query heads of a request,
+// a warp each, or (many parts, or heads too few to fill the GPU) one at a time, its warps sharing the parts.
 constexpr int kMergeWarps = 8;
 template <int HD>
-__device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, int64_t slot0, int begin, int step, int n,
+__device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, int64_t slot0, int begin, int end,
                                             float& m, float& l, float (&acc)[HD / 32]) {
   constexpr int E = HD / 32, V = E < 4 ? E : 4, kFly = 64 / E;
   const int lane = threadIdx.x & 31;
   auto row = [&](int i) { return row0 + static_cast<int64_t>(i) * 2 * P.hq + (i == 0 ? slot0 : 0); };
+  float x[kFly][E];
+  auto load = [&](int i0, int n) {
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      if (k >= n) break;
+      const float* src = P.part_acc + row(i0 + k) * HD + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e += V) {
+        if constexpr (V == 2)
+          *reinterpret_cast<float2*>(&x[k][e]) = __ldcg(reinterpret_cast<const float2*>(src + e));
+        else
+          *reinterpret_cast<float4*>(&x[k][e]) = __ldcg(reinterpret_cast<const float4*>(src + e));
+      }
+    }
+  };
   m = -INFINITY;
   l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i0 = begin; i0 < n; i0 += step) {
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int here = min(32, end - i0);
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (i0 + lane < n) ml = __ldcg(reinterpret_cast<const float2*>(P.part_ml) + row(i0 + lane));
+    if (lane < here) ml = __ldcg(reinterpret_cast<const float2*>(P.part_ml) + row(i0 + lane));
+    load(i0, here);
     const float top = fmaxf(m, warp_max(ml.x));
     const float down = l == 0.f ? 0.f : exp2f(m - top);
     const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - top);  // no tokens: nothing (a NaN goes on)
@@ -207,21 +226,8 @@ __device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, i
     m = top;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= down;
-    const int here = min(32, n - i0);
     for (int j = 0; j < here; j += kFly) {
-      float x[kFly][E];
-#pragma unroll
-      for (int k = 0; k < kFly; ++k) {
-        if (j + k >= here) break;
-        const float* src = P.part_acc + row(i0 + j + k) * HD + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e += V) {
-          if constexpr (V == 2)
-            *reinterpret_cast<float2*>(&x[k][e]) = __ldcg(reinterpret_cast<const float2*>(src + e));
-          else
-            *reinterpret_cast<float4*>(&x[k][e]) = __ldcg(reinterpret_cast<const float4*>(src + e));
-        }
-      }
+      if (j > 0) load(i0 + j, here - j);
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
         if (j + k >= here) break;
@@ -234,21 +240,25 @@ __device__ __forceinline__ void merge_parts(const AttnParams& P, int64_t row0, i
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __grid_constant__ AttnParams P) {
+__global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __grid_constant__ AttnParams P,
+                                                                     int heads_cta) {
   constexpr int E = HD / 32;
   __shared__ float red[kMergeWarps][HD + 2];
-  const int b = blockIdx.y, h_begin = blockIdx.x * kMergeWarps, h_end = min(P.hq, h_begin + kMergeWarps);
+  const int b = blockIdx.y, h_begin = blockIdx.x * heads_cta, h_end = min(P.hq, h_begin + heads_cta);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 parts = __ldcg(&P.parts[b]);
   const int n = parts.y;
   if (n == 1) return;  // written by its one CTA
   const int64_t row0 = static_cast<int64_t>(parts.x & ~1) * P.hq, slot0 = (parts.x & 1) * P.hq;
-  const bool few = n <= 64;
-  for (int h = h_begin + (few ? warp : 0); h < h_end; h += few ? kMergeWarps : 1) {
+  const bool apart = heads_cta > 1 && n <= 64;
+  const int each = apart ? n : (n + kMergeWarps - 1) / kMergeWarps;
+  const int begin = apart ? 0 : warp * each, end = min(n, begin + each);
+  for (int h = h_begin + (apart ? warp : 0); h < h_end; h += apart ? kMergeWarps : 1) {
     float m, l, acc[E];
-    merge_parts<HD>(P, row0 + h, slot0, few ? 0 : warp * 32, few ? 32 : kMergeWarps * 32, n, m, l, acc);
-    if (!few) {
+    merge_parts<HD>(P, row0 + h, slot0, begin, end, m, l, acc);
+    if (!apart) {
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < E; ++e) red[warp][lane * E + e] = acc[e];
@@ -310,6 +320,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map)) : "memory");
   }
 
+  // What is above overlaps the end of the kernel before; nothing that it may have written is read above.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // ---- this CTA's range of rounds, and the request it begins in
   __shared__ int64_t warp_sum[kMaxWarps];
   __shared__ int64_t start_first;
@@ -368,9 +380,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   while (f < f_end) {
     const int seq = tokens_of(P, b);
     const int rounds = rounds_of(seq, P.streams);
-    const int r0 = static_cast<int>(f - first);
-    const int mine = static_cast<int>(min(static_cast<int64_t>(rounds), f_end - first)) - r0;  // tiles of this warp here
-    const bool whole_request = mine == rounds;
+    const int r_begin = static_cast<int>(f - first);
+    const int r_end = static_cast<int>(min(static_cast<int64_t>(rounds), f_end - first));
+    const bool whole_request = r_begin == 0 && r_end == rounds;
+    const int r0 = max(r_begin - kStart, 0);
+    const int mine = r_end - kStart - r0;  // tiles of this warp here (not positive: only the request's start is)
     const int t_begin = r0 * round_tokens + stream * kTile;  // tile i begins at t_begin + i round_tokens
     const int32_t* table = P.table + b * P.table_stride;
 
@@ -430,17 +444,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         return live;
       }
     };
-    uint32_t next = issue(0);
-
     // ---- q as operands: column gid is head gid / 2, odd columns the second parts (PAIR), or head gid
+    uint32_t next;
     uint32_t bq[NG][2][2], bz[NZ][2];
     float factor[NH];
     {
       const int h = PAIR ? gid >> 1 : gid;
       const bool second = PAIR && (gid & 1) != 0;
       uint32_t xw[NG][4];
-      float top = 0.f;
-      bool bad = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         int4 w = make_int4(0, 0, 0, 0);
@@ -448,12 +459,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           w = *reinterpret_cast<const int4*>(P.q + b * P.q_stride + (head0 + h) * static_cast<int64_t>(HD) +
                                              g * kGroup + tig * 8);
         xw[g][0] = w.x, xw[g][1] = w.y, xw[g][2] = w.z, xw[g][3] = w.w;
+      }
+      next = issue(0);  // behind the loads of q: both are under way together
+      float top = 0.f;
+      bool bad = false;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           top = fmaxf(top, fmaxf(fabsf(bf_lo(xw[g][k])), fabsf(bf_hi(xw[g][k]))));
           bad |= (xw[g][k] & 0x7f80u) == 0x7f80u || (xw[g][k] & 0x7f800000u) == 0x7f800000u;
         }
-      }
       int flag = bad;
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
@@ -825,12 +841,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           P.part_ml[(slot_row + h) * 2 + 1] = l[n];
         }
       }
-      if (r0 == 0 && y == 0 && lane == 0)
+      if (r_begin == 0 && y == 0 && lane == 0)
         P.parts[b] = make_int2(2 * blockIdx.x + (f == f_begin ? 0 : 1),
                                static_cast<int>((first + rounds - 1) / per) - static_cast<int>(blockIdx.x) + 1);
     }
-    f = first + r0 + mine;
-    if (r0 + mine == rounds) {
+    f = first + r_end;
+    if (r_end == rounds) {
       first += rounds;
       ++b;
     }
@@ -884,6 +900,22 @@ inline bool make_map(CUtensorMap* map, const Cache& c, int row) {
          CUDA_SUCCESS;
 }
 
+// Lets a kernel be put in place before the one in front of it has ended; it waits for that itself.
+template <typename K, typename... A>
+cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int HD, bool PAIR, bool TMA>
 cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, const Plan& plan, cudaStream_t stream) {
   auto kernel = kv4_decode_kernel<HD, PAIR, TMA>;
@@ -892,8 +924,7 @@ cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, co
   const int smem = warps * std::max(Geometry<HD>::kRingBytes, kVals * 128);
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<dim3(plan.ctas, plan.y_ctas), warps * 32, smem, stream>>>(P, map);
-  return cudaGetLastError();
+  return launch_overlapped(kernel, dim3(plan.ctas, plan.y_ctas), warps * 32, smem, stream, P, map);
 }
 
 template <int HD>
@@ -908,16 +939,9 @@ cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t
     e = tma ? launch_decode_kernel<HD, false, true>(P, map, plan, stream)
             : launch_decode_kernel<HD, false, false>(P, map, plan, stream);
   if (e != cudaSuccess || plan.ctas == 1) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((P.hq + kMergeWarps - 1) / kMergeWarps, P.batch);
-  cfg.blockDim = dim3(kMergeWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<HD>, P);
+  const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 2 * 148 ? 1 : kMergeWarps;
+  return launch_overlapped(kv4_merge_kernel<HD>, dim3((P.hq + heads_cta - 1) / heads_cta, P.batch), kMergeWarps * 32, 0,
+                           stream, P, heads_cta);
 }
 
 inline cudaError_t launch_decode(const AttnParams& P, int hd, const Plan& plan, cudaStream_t stream) {

@@ -9,6 +9,11 @@ prefill attention to PyTorch SDPA (flash / cuDNN backends only), and the
 fused ops (RMSNorm+residual, RoPE+paged KV write, SiLU-mul, paged decode
 attention) to the sm_100a kernels in ``libkvbm_cuda.so``.
 
+A pool from ``allocate_pool(..., kv_bits=4)`` holds K and V in 4 bits: the
+writes quantise, decode attends over the codes, and a cached prefix is read
+back as bf16 for the prefill attention. With ``LlamaConfig.qk_norm`` every q
+and k head is RMS-normalised before the rotation.
+
 The reference ships no model (vLLM provides it there); this harness plays
 vLLM's role for the benchmarks, calling the same connector hooks.
 """
@@ -23,7 +28,7 @@ import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 from torch.nn.attention.bias import causal_lower_right
 
-from ..ops import llama_ops
+from ..ops import kv4_ops, llama_ops, table_ops
 from ..physical.layout import KvBlockLayout, KvLayout, LayoutConfig
 
 
@@ -39,6 +44,7 @@ class LlamaConfig:
     rope_theta: float = 500000.0
     eps: float = 1e-5
     max_position: int = 16384
+    qk_norm: bool = False  # RMS norm of every q and k head before the rotation
 
     @classmethod
     def llama3_8b(cls) -> "LlamaConfig":
@@ -59,7 +65,9 @@ class LlamaConfig:
 
     def kv_layout_config(self, num_blocks: int, page_size: int = 16,
                          dtype: torch.dtype = torch.bfloat16) -> LayoutConfig:
-        return LayoutConfig.for_model(num_blocks, self.layers, self.kv_heads, self.head_dim, page_size, dtype)
+        """``dtype`` uint8: a 4-bit pool, whose rows are bytes."""
+        row = kv4_ops.row_bytes(self.head_dim) if dtype == torch.uint8 else self.head_dim
+        return LayoutConfig.for_model(num_blocks, self.layers, self.kv_heads, row, page_size, dtype)
 
     def num_params(self) -> int:
         per_layer = (self.hidden * (self.q_size + 2 * self.kv_size) + self.q_size * self.hidden
@@ -191,6 +199,8 @@ class LlamaModel:
                 "wqkv": wqkv, "wo": wo, "wgu": wgu, "wd": wd,
                 "n1": torch.ones(c.hidden, device=self.device, dtype=dtype),
                 "n2": torch.ones(c.hidden, device=self.device, dtype=dtype),
+                "qn": torch.ones(c.head_dim, device=self.device, dtype=dtype) if c.qk_norm else None,
+                "kn": torch.ones(c.head_dim, device=self.device, dtype=dtype) if c.qk_norm else None,
             })
         self.norm = torch.ones(c.hidden, device=self.device, dtype=dtype)
         self.lm_head = torch.empty(c.vocab, c.hidden, device=self.device, dtype=dtype).normal_(0.0, std,
@@ -220,8 +230,11 @@ class LlamaModel:
         return k, k + pool.outer_stride
 
     def allocate_pool(self, num_blocks: int, page_size: int = 16, kind: str = "fully_contiguous",
-                      block_layout: KvBlockLayout = KvBlockLayout.OPERATIONAL_NHD) -> KvLayout:
-        return KvLayout.allocate(self.cfg.kv_layout_config(num_blocks, page_size), kind, block_layout,
+                      block_layout: KvBlockLayout = KvBlockLayout.OPERATIONAL_NHD, kv_bits: int = 16) -> KvLayout:
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, not {kv_bits}")
+        dtype = torch.uint8 if kv_bits == 4 else torch.bfloat16
+        return KvLayout.allocate(self.cfg.kv_layout_config(num_blocks, page_size, dtype), kind, block_layout,
                                  device=self.device.index)
 
     # ------------------------------------------------------------ prefill
@@ -245,7 +258,15 @@ class LlamaModel:
         T = tokens.numel()
         page = pool.config.page_size
         pos = torch.arange(start_pos, start_pos + T, device=self.device, dtype=torch.int32)
-        slots = (block_ids.long()[pos.long() // page] * page + pos.long() % page)
+        block_ids = block_ids.to(torch.int32).contiguous()
+        slots = table_ops.slot_map(block_ids, pos, page=page)
+        kv4 = pool.dtype == torch.uint8
+        if kv_push is not None and (kv4 or c.qk_norm):
+            raise ValueError("the fused push takes 16-bit pools of models without q/k head norms")
+        prefix = None
+        if kv4 and start_pos > 0:
+            prefix = table_ops.slot_map(block_ids, torch.arange(start_pos, device=self.device, dtype=torch.int32),
+                                        page=page)
         x = F.embedding(tokens.long(), self.embed)
         residual = x
         h = torch.empty_like(x)
@@ -260,7 +281,10 @@ class LlamaModel:
                 llama_ops.rmsnorm(x, L["n1"], c.eps, residual=residual, out=h)
             qkv = F.linear(h, L["wqkv"]).view(T, c.heads + 2 * c.kv_heads, c.head_dim)
             kb, vb = self.kv_bases(pool, li)
-            if kv_push is None:
+            if kv4 or c.qk_norm:
+                kv4_ops.qk_norm_rope_kv_write(qkv, pos, self.cos_sin, c.heads, c.kv_heads, pool.layer_view(li), slots,
+                                              q_weight=L["qn"], k_weight=L["kn"], eps=c.eps)
+            elif kv_push is None:
                 llama_ops.rope_kv_write(qkv, pos, self.cos_sin, c.heads, c.kv_heads, c.head_dim, kb, vb,
                                         pool.block_stride, pool.token_stride, pool.head_stride, page, slots)
             else:
@@ -273,10 +297,13 @@ class LlamaModel:
             v = qkv[:, c.heads + c.kv_heads:].transpose(0, 1)
             if start_pos > 0:
                 # cached prefix (e.g. onboarded from G2): read its K/V from the pool
-                nb = (start_pos + page - 1) // page
-                view = pool.layer_view(li)[block_ids[:nb].long()]  # [nb, 2, page, Hkv, D]
-                pk = view[:, 0].reshape(-1, c.kv_heads, c.head_dim)[:start_pos].transpose(0, 1)
-                pv = view[:, 1].reshape(-1, c.kv_heads, c.head_dim)[:start_pos].transpose(0, 1)
+                if kv4:
+                    pk, pv = (t.transpose(0, 1) for t in kv4_ops.kv4_gather(pool.layer_view(li), prefix))
+                else:
+                    nb = (start_pos + page - 1) // page
+                    view = pool.layer_view(li)[block_ids[:nb].long()]  # [nb, 2, page, Hkv, D]
+                    pk = view[:, 0].reshape(-1, c.kv_heads, c.head_dim)[:start_pos].transpose(0, 1)
+                    pv = view[:, 1].reshape(-1, c.kv_heads, c.head_dim)[:start_pos].transpose(0, 1)
                 k = torch.cat([pk, k], dim=1)
                 v = torch.cat([pv, v], dim=1)
             a = self._attention(q, k.unsqueeze(0), v.unsqueeze(0), start_pos)
@@ -331,7 +358,9 @@ class LlamaModel:
 
     # ------------------------------------------------------------- decode
     def decode_scratch(self, batch: int, splits: int) -> torch.Tensor:
-        need = batch * self.cfg.heads * splits * (self.cfg.head_dim + 2)
+        return self._scratch(batch * self.cfg.heads * splits * (self.cfg.head_dim + 2))
+
+    def _scratch(self, need: int) -> torch.Tensor:
         if self._decode_scratch is None or self._decode_scratch.numel() < need:
             self._decode_scratch = torch.empty(need, dtype=torch.float32, device=self.device)
         return self._decode_scratch
@@ -358,17 +387,22 @@ class LlamaModel:
         """One decode step for a batch: tokens [B] int64, positions [B] int32
         (position of each input token), block_table [B, max_blocks] int32,
         seq_lens [B] int32 (= positions + 1). Returns next tokens [B] int64.
-        All shapes static, so the step can be captured in a CUDA graph."""
+        All shapes static, so the step can be captured in a CUDA graph.
+        ``splits`` is for 16-bit pools; over 4 bits the work is cut evenly on the device."""
         c = self.cfg
         B = tokens.numel()
         page = pool.config.page_size
-        pl = positions.long()
-        slots = block_table.gather(1, (pl // page).unsqueeze(1)).squeeze(1).long() * page + pl % page
+        slots = table_ops.slot_map(block_table, positions, page=page)
         x = F.embedding(tokens, self.embed)
         residual = x
         h = torch.empty_like(x)
-        scratch = self.decode_scratch(B, splits)
-        counters = self.decode_counters(B)
+        kv4 = pool.dtype == torch.uint8
+        if kv4:
+            scratch = self._scratch(kv4_ops.kv4_decode_scratch(B, c.heads, c.kv_heads, c.head_dim,
+                                                               block_table.shape[1] * page, device=self.device))
+        else:
+            scratch = self.decode_scratch(B, splits)
+            counters = self.decode_counters(B)
         attn = torch.empty(B, c.heads, c.head_dim, device=self.device, dtype=self.dtype)
         q = torch.empty(B, c.heads, c.head_dim, device=self.device, dtype=self.dtype)
         for li, L in enumerate(self.layers):
@@ -378,16 +412,23 @@ class LlamaModel:
                 llama_ops.rmsnorm(x, L["n1"], c.eps, residual=residual, out=h)
             qkv = self.dlinear(h, L["wqkv"]).view(B, c.heads + 2 * c.kv_heads, c.head_dim)
             kb, vb = self.kv_bases(pool, li)
-            if c.head_dim == 128:
+            if kv4 or c.qk_norm:
+                view = pool.layer_view(li)
+                kv4_ops.qk_norm_rope_kv_write(qkv, positions, self.cos_sin, c.heads, c.kv_heads, view, slots,
+                                              q_weight=L["qn"], k_weight=L["kn"], eps=c.eps, q_out=q)
+            elif c.head_dim == 128:
                 llama_ops.rope_kv_write_qout(qkv, positions, self.cos_sin, c.heads, c.kv_heads, kb, vb,
                                              pool.block_stride, pool.token_stride, pool.head_stride, page, slots, q)
             else:
                 llama_ops.rope_kv_write(qkv, positions, self.cos_sin, c.heads, c.kv_heads, c.head_dim, kb, vb,
                                         pool.block_stride, pool.token_stride, pool.head_stride, page, slots)
                 q.copy_(qkv[:, : c.heads])
-            llama_ops.paged_decode_attn(q, kb, vb, pool.block_stride, pool.token_stride, pool.head_stride, page,
-                                        block_table, seq_lens, c.kv_heads, self.scale, splits, scratch=scratch,
-                                        out=attn, counters=counters)
+            if kv4:
+                kv4_ops.paged_decode_attn_kv4(q, view, block_table, seq_lens, self.scale, scratch=scratch, out=attn)
+            else:
+                llama_ops.paged_decode_attn(q, kb, vb, pool.block_stride, pool.token_stride, pool.head_stride, page,
+                                            block_table, seq_lens, c.kv_heads, self.scale, splits, scratch=scratch,
+                                            out=attn, counters=counters)
             x = self._reduce(self.dlinear(attn.view(B, c.q_size), L["wo"]))
             llama_ops.rmsnorm(x, L["n2"], c.eps, residual=residual, out=h)
             x = self._reduce(self.dlinear(llama_ops.silu_mul(self.dlinear(h, L["wgu"])), L["wd"]))
@@ -416,8 +457,10 @@ class LlamaModel:
         for L in self.layers:
             hN = norm(x, L["n1"])
             qkv = (hN @ L["wqkv"].float().t()).view(T, -1, c.head_dim)
-            q = rope(qkv[:, : c.heads])
-            k = rope(qkv[:, c.heads: c.heads + c.kv_heads])
+            q, k = qkv[:, : c.heads], qkv[:, c.heads: c.heads + c.kv_heads]
+            if c.qk_norm:
+                q, k = norm(q, L["qn"]), norm(k, L["kn"])
+            q, k = rope(q), rope(k)
             v = qkv[:, c.heads + c.kv_heads:]
             rep = c.heads // c.kv_heads
             k = k.repeat_interleave(rep, dim=1)

@@ -94,6 +94,8 @@ def kv_transfer(src, src_ids, dst, dst_ids, *, layer_begin: int = 0, num_layers:
     nh = num_heads if num_heads is not None else min(sc.num_heads - src_head_offset, dc.num_heads - dst_head_offset)
     if src_head_offset + nh > sc.num_heads or dst_head_offset + nh > dc.num_heads:
         raise ValueError("head slice out of range")
+    if src.dtype != dst.dtype and torch.uint8 in (src.dtype, dst.dtype):
+        raise ValueError("a pool of bytes (a 4-bit cache) is copied to pools of bytes only, not cast")
     if sc.head_dim != dc.head_dim or sc.page_size != dc.page_size or sc.outer_dim != dc.outer_dim:
         raise ValueError("pools differ in head_dim, page_size or outer_dim")
     dev = torch.device("cuda", torch.cuda.current_device())

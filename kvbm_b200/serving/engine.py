@@ -44,7 +44,7 @@ from ..connector.worker import ConnectorWorker
 from ..logical.manager import BlockManager, MutableBlock, Tier
 from ..logical.sequence import sequence_hashes
 from ..models.llama import LlamaModel
-from ..ops import llama_ops
+from ..ops import llama_ops, table_ops
 from ..physical.layout import KvLayout
 
 
@@ -99,6 +99,7 @@ class EngineConfig:
     record_events: bool = True           # arrival / first-token CUDA events per request
     max_inflight_steps: int = 2          # the host runs at most this many steps ahead of the GPU
     prefix_caching: bool = False         # keep finished prompts' full blocks in G1 (LRU) and match them first
+    kv_bits: int = 16                    # 4: the engine's pool holds K/V in 4 bits (a connector's tiers then hold bytes)
 
 
 class DecodeBatch:
@@ -169,17 +170,26 @@ class DecodeBatch:
             return
         n = len(entries)
         dev = self.tok.device
-        slots = torch.tensor([e[0] for e in entries], dtype=torch.int64)
-        rows = torch.full((n, self.max_blocks), self.dummy, dtype=torch.int32)
-        for i, e in enumerate(entries):
+        for e in entries:
             if len(e[1]) > self.max_blocks:
                 raise ValueError(f"{len(e[1])} blocks exceed the decode batch's {self.max_blocks}")
-            rows[i, : len(e[1])] = torch.tensor(e[1], dtype=torch.int32)
-        scal = torch.tensor([[e[2], e[3], e[3] + 1, e[4]] for e in entries], dtype=torch.int64)
-        slots_d = slots.pin_memory().to(dev, non_blocking=True)
-        rows_d = rows.pin_memory().to(dev, non_blocking=True)
+        scal = torch.tensor([[e[2], e[3], e[3] + 1, e[4], e[0]] for e in entries], dtype=torch.int64)
         scal_d = scal.pin_memory().to(dev, non_blocking=True)
-        self.block_table.index_copy_(0, slots_d, rows_d)
+        slots_d = scal_d[:, 4]
+        if dev.type == "cuda":
+            # the entering requests' lengths and blocks go up as they are; their table rows are built on the device
+            flat = [e[0] for e in entries] + [e[3] for e in entries] + [len(e[1]) for e in entries] + [1] * n
+            for e in entries:
+                flat += e[1]
+            up = torch.tensor(flat, dtype=torch.int32).pin_memory().to(dev, non_blocking=True)
+            rows, ctx, counts, query, ids = up.split([n, n, n, n, up.numel() - 4 * n])
+            table_ops.batch_tables(query, ctx, ids, page=self.pool.config.page_size, block_counts=counts,
+                                   table=self.block_table, rows=rows, pad_block=self.dummy)
+        else:
+            rows = torch.full((n, self.max_blocks), self.dummy, dtype=torch.int32)
+            for i, e in enumerate(entries):
+                rows[i, : len(e[1])] = torch.tensor(e[1], dtype=torch.int32)
+            self.block_table.index_copy_(0, slots_d, rows)
         keep = scal_d[:, 0] < 0
         self.tok.index_copy_(0, slots_d, torch.where(keep, self.tok.index_select(0, slots_d), scal_d[:, 0]))
         self.pos.index_copy_(0, slots_d, scal_d[:, 1].to(torch.int32))
@@ -242,7 +252,10 @@ class LLMEngine:
                  worker: ConnectorWorker | None = None, pool: KvLayout | None = None, tp=None):
         self.model, self.cfg = model, cfg
         self.device = model.device
-        self.pool = pool if pool is not None else model.allocate_pool(cfg.num_gpu_blocks, cfg.block_size)
+        if pool is None:
+            bits = {} if cfg.kv_bits == 16 else {"kv_bits": cfg.kv_bits}
+            pool = model.allocate_pool(cfg.num_gpu_blocks, cfg.block_size, **bits)
+        self.pool = pool
         self.tp = tp
         self.is_scheduler = tp is None or tp.rank == 0
         self.leader, self.worker = (leader if self.is_scheduler else None), worker

@@ -80,6 +80,7 @@ struct AttnParams {
   float* part_ml;   // [cta][2][hq][2]
   int2* parts;      // [batch]: a request's first slot of partial results (2 cta, + 1: not its CTA's first), and how many
   __nv_bfloat16* out;
+  bool flat;  // a head's rows in a page are contiguous: the copies take them as one
 };
 
 constexpr int kHeads = 8;       // query heads a warp takes at most
@@ -137,13 +138,13 @@ __device__ __forceinline__ void lds(uint32_t (&x)[WORDS], uint32_t addr) {
                    : "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3])
                    : "r"(addr + 4 * i));
 }
-// K and V rows of `kUnit` tokens of one KV head: coordinates (byte, head, token in the page, K / V, block).
-__device__ __forceinline__ void copy_unit(uint32_t smem, const CUtensorMap* map, int head, int token, int block,
+// K and V rows of `kUnit` tokens of one KV head: coordinates (byte / 8, head, token in the page, K / V, block).
+__device__ __forceinline__ void copy_unit(uint32_t smem, const CUtensorMap* map, int word, int head, int token, int block,
                                           uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
       "[%7];" ::"r"(smem),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(head), "r"(token), "r"(0), "r"(block), "r"(smem_u32(bar))
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(word), "r"(head), "r"(token), "r"(0), "r"(block), "r"(smem_u32(bar))
       : "memory");
 }
 __device__ __forceinline__ uint32_t half2(float lo, float hi) {
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         if (two != 0u && (lane >> 1) == (tile & 15)) {
           uint64_t* bar = &full[warp][tile & 1];
           mbar_arrive_expect_tx(bar, id >= 0 ? G::kUnitBytes : 0);
-          if (id >= 0) copy_unit(st + (lane & 1) * G::kUnitBytes, &map, kvh, at, id, bar);
+          if (id >= 0) copy_unit(st + (lane & 1) * G::kUnitBytes, &map, P.flat ? at * (G::kRow / 8) : 0, kvh, P.flat ? 0 : at, id, bar);
         }
         return two;
       } else {  // every row looks its own page up
@@ -877,8 +878,10 @@ inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, 
   return p;
 }
 
-// The pool as a tensor of bytes [block][K / V][token][head][row], boxes of a unit's rows of one head.
-inline bool make_map(CUtensorMap* map, const Cache& c, int row) {
+// The pool as a tensor of 8-byte words [block][K / V][token][head][row], boxes of a unit's rows of one head. Where a
+// head's rows of a page are contiguous (head-first pools) and a unit's are no longer than a box may be, the tokens
+// are part of the innermost dimension: 2 runs a box instead of 32.
+inline bool make_map(CUtensorMap* map, const Cache& c, int row, bool* flat) {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -887,15 +890,18 @@ inline bool make_map(CUtensorMap* map, const Cache& c, int row) {
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? p : nullptr);
   }();
   if (!fn || c.num_blocks < 1) return false;
-  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(row), static_cast<cuuint64_t>(c.heads),
-                              static_cast<cuuint64_t>(c.page), 2, static_cast<cuuint64_t>(c.num_blocks)};
+  *flat = c.token_stride == row && kUnit * row / 8 <= 256;
+  const cuuint64_t words = static_cast<cuuint64_t>(row) / 8;
+  const cuuint64_t dims[5] = {*flat ? words * c.page : words, static_cast<cuuint64_t>(c.heads),
+                              *flat ? 1 : static_cast<cuuint64_t>(c.page), 2, static_cast<cuuint64_t>(c.num_blocks)};
   // a dimension of one may come with any stride
   const cuuint64_t strides[4] = {static_cast<cuuint64_t>(c.heads > 1 ? c.head_stride : row),
                                  static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.outer_stride),
                                  static_cast<cuuint64_t>(c.num_blocks > 1 ? c.block_stride : row)};
-  const cuuint32_t box[5] = {static_cast<cuuint32_t>(row), 1, kUnit, 2, 1};
+  const cuuint32_t box[5] = {static_cast<cuuint32_t>(*flat ? words * kUnit : words), 1,
+                             static_cast<cuuint32_t>(*flat ? 1 : kUnit), 2, 1};
   const cuuint32_t step[5] = {1, 1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, c.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 5, c.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
          CUDA_SUCCESS;
 }
@@ -928,9 +934,9 @@ cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, co
 }
 
 template <int HD>
-cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t stream) {
+cudaError_t launch_decode_hd(AttnParams& P, const Plan& plan, cudaStream_t stream) {
   CUtensorMap map{};
-  const bool tma = P.cache.page % kUnit == 0 && make_map(&map, P.cache, row_bytes(HD));
+  const bool tma = P.cache.page % kUnit == 0 && make_map(&map, P.cache, row_bytes(HD), &P.flat);
   cudaError_t e;
   if (P.group <= 4)
     e = tma ? launch_decode_kernel<HD, true, true>(P, map, plan, stream)
@@ -944,7 +950,7 @@ cudaError_t launch_decode_hd(const AttnParams& P, const Plan& plan, cudaStream_t
                            stream, P, heads_cta);
 }
 
-inline cudaError_t launch_decode(const AttnParams& P, int hd, const Plan& plan, cudaStream_t stream) {
+inline cudaError_t launch_decode(AttnParams& P, int hd, const Plan& plan, cudaStream_t stream) {
   switch (hd) {
     case 64: return launch_decode_hd<64>(P, plan, stream);
     case 128: return launch_decode_hd<128>(P, plan, stream);

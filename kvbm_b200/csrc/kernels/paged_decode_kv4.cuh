@@ -51,7 +51,11 @@
 // Copies. Each warp has its own ring of two tiles. A unit of 16 tokens, K and V
 // rows of one KV head, is one TMA box of the five-dimensional pool, issued by the
 // lane that looked the unit's page up (32 units at a time); where a page is not a
-// multiple of 16 tokens, rows are copied one by one with cp.async.
+// multiple of 16 tokens, rows are copied one by one with cp.async. What limits the
+// copies is the number of contiguous runs, of 80 bytes with 128 elements a head:
+// in a head-first pool the 16 rows are one run, and in a token-first one two warps
+// share the rows of two neighbouring heads (SHARED), one of them issuing, with a
+// barrier of the two where a tile's stage is given back.
 #pragma once
 
 #include "common.cuh"
@@ -85,9 +89,9 @@ struct AttnParams {
 
 constexpr int kHeads = 8;       // query heads a warp takes at most
 constexpr int kMaxWarps = 8;
+enum Copies { kRows, kTma, kTmaShared };
 constexpr int kUnit = 16;       // tokens a stage of the ring holds
 constexpr int kTile = 32;       // tokens a warp takes between two updates of its accumulators
-constexpr int kStages = 4;      // two tiles of two units
 constexpr int kMinRounds = 2;   // a CTA takes at least so many tiles a warp: below, merging costs more than it saves
 constexpr uint64_t kWaitNs = 1000000000ull;  // after which a warp gives a copy up
 
@@ -296,15 +300,17 @@ struct Geometry {
   static constexpr int NG = HD / kGroup;
   static constexpr int kRow = row_bytes(HD);
   static constexpr int kChunks = kRow / 16;        // 16-byte pieces a row; also copies a lane for a unit
-  static constexpr int kUnitBytes = 2 * kUnit * kRow;  // K rows, then V rows
   static constexpr int kCtasPerSm = HD == 256 ? 1 : 2;  // of 8 warps
-  static constexpr int kRingBytes = kStages * kUnitBytes;  // a warp
+  static constexpr int kRingBytes = 4 * 2 * kUnit * kRow;  // a warp: two tiles of two units, K and V
 };
 
-template <int HD, bool PAIR, bool TMA>
+template <int HD, bool PAIR, Copies COPIES>
 __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     kv4_decode_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map) {
   using G = Geometry<HD>;
+  constexpr bool TMA = COPIES != kRows, SHARED = COPIES == kTmaShared;
+  constexpr int kStride = SHARED ? 2 * G::kRow : G::kRow;  // between rows in shared memory
+  constexpr int kStage = 2 * kUnit * kStride;              // a unit's K rows, then its V rows
   constexpr int NG = G::NG;
   constexpr int NH = PAIR ? 1 : 2;       // query heads whose scores a lane holds
   constexpr int NW = NG / 2;             // words of V codes a lane takes from a row
@@ -373,7 +379,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   const int heads = active ? min(kHeads, P.group - h0) : 0;
   const int head0 = kvh * P.group + h0;  // first query head
 
-  const uint32_t ring = smem_u32(smem) + warp * G::kRingBytes;
+  // Two warps that share copies are 2 k and 2 k + 1; they have both their rings and one set of barriers.
+  const bool leads = !SHARED || (warp & 1) == 0;
+  const int owner = SHARED ? warp & ~1 : warp;
+  const uint32_t ring = smem_u32(smem) + owner * G::kRingBytes;
+  const uint32_t mine_at = SHARED ? (warp & 1) * G::kRow : 0;  // this warp's head in a row
+  auto give_back = [&] {  // the stage just read may be written
+    if constexpr (SHARED)
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+    else
+      __syncwarp();
+  };
   const int round_tokens = kTile * P.streams;
   uint32_t phases = 0u;  // of full[warp][0], [1]
   bool given_up = false;
@@ -394,12 +410,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     int32_t id = -1, at = 0;    // block of the unit that this lane looked up and its first token there
     uint32_t there = 0u;        // which of the 32 units have a block
     auto issue = [&](int tile) {
-      if (tile >= mine || !active || given_up) {
+      if (tile >= mine || !active) {
         if constexpr (!TMA) copy_commit();
         return 0u;
       }
       const int t0 = t_begin + tile * round_tokens;
-      const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
+      const uint32_t st = ring + (tile & 1) * 2 * kStage;
       if constexpr (TMA) {
         if ((tile & 15) == 0) {  // the next 32 units, one a lane
           const int t = t_begin + (tile + (lane >> 1)) * round_tokens + (lane & 1) * kUnit;
@@ -413,10 +429,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           there = __ballot_sync(0xffffffffu, id >= 0);
         }
         const uint32_t two = (there >> (2 * (tile & 15))) & 3u;
-        if (two != 0u && (lane >> 1) == (tile & 15)) {
-          uint64_t* bar = &full[warp][tile & 1];
-          mbar_arrive_expect_tx(bar, id >= 0 ? G::kUnitBytes : 0);
-          if (id >= 0) copy_unit(st + (lane & 1) * G::kUnitBytes, &map, P.flat ? at * (G::kRow / 8) : 0, kvh, P.flat ? 0 : at, id, bar);
+        if (two != 0u && leads && !given_up && (lane >> 1) == (tile & 15)) {
+          uint64_t* bar = &full[owner][tile & 1];
+          mbar_arrive_expect_tx(bar, id >= 0 ? kStage : 0);
+          if (id >= 0) copy_unit(st + (lane & 1) * kStage, &map, P.flat ? at * (G::kRow / 8) : 0, SHARED ? kvh >> 1 : kvh, P.flat ? 0 : at, id, bar);
         }
         return two;
       } else {  // every row looks its own page up
@@ -437,7 +453,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
             const int32_t blk = __shfl_sync(0xffffffffu, row_block, u * kUnit + r);
             const int32_t off = __shfl_sync(0xffffffffu, row_at, u * kUnit + r);
             if (blk >= 0)
-              copy16(st + u * G::kUnitBytes + c * 16,
+              copy16(st + u * kStage + c * 16,
                      P.cache.base + blk * P.cache.block_stride + (v ? P.cache.outer_stride : 0) +
                          off * P.cache.token_stride + kvh * P.cache.head_stride + piece * 16);
           }
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       m[n] = -INFINITY;
-      l[n] = given_up ? __uint_as_float(0x7fc00000u) : 0.f;
+      l[n] = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         z[n][g] = 0.f;
@@ -551,23 +567,27 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       }
       if (here == 0u) continue;
       if constexpr (TMA) {
-        const int k = tile & 1;
-        bool ok = mbar_try_wait(&full[warp][k], (phases >> k) & 1u);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
-          if (!__all_sync(0xffffffffu, ok)) {  // leave, when both copies in flight have ended or are given up
-            given_up = true;
-            report_status(&g_kv4_status, kStatusPipelineTimeout);
-            mbar_wait_bounded(&full[warp][k], (phases >> k) & 1u, kWaitNs);
-            if (next != 0u) mbar_wait_bounded(&full[warp][k ^ 1], (phases >> (k ^ 1)) & 1u, kWaitNs);
-#pragma unroll
-            for (int n = 0; n < NH; ++n) l[n] = __uint_as_float(0x7fc00000u);
-            break;
+        if (!given_up) {
+          uint64_t* bar = &full[owner][tile & 1];
+          const uint32_t phase = (phases >> (tile & 1)) & 1u;
+          bool ok = mbar_try_wait(bar, phase);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = mbar_wait_bounded(bar, phase, kWaitNs);
+            if (!__all_sync(0xffffffffu, ok)) {  // the launch is given up when both copies in flight have had their time
+              given_up = true;
+              report_status(&g_kv4_status, kStatusPipelineTimeout);
+              mbar_wait_bounded(bar, phase, kWaitNs);
+              if (next != 0u) mbar_wait_bounded(&full[owner][~tile & 1], (phases >> (~tile & 1)) & 1u, kWaitNs);
+            }
           }
+          phases ^= 1u << (tile & 1);
         }
-        phases ^= 1u << k;
+        if (given_up) {  // no more copies, no more waiting; the results are NaN
+          give_back();
+          continue;
+        }
       }
-      const uint32_t st = ring + (tile & 1) * 2 * G::kUnitBytes;
+      const uint32_t st = ring + (tile & 1) * 2 * kStage + mine_at;
       const int left = seq - (t_begin + tile * round_tokens);  // tokens from this tile's first on, at least 1
       const bool whole = here == (TMA ? 3u : 0xffffffffu) && left >= kTile;
       uint32_t live = 0xffffffffu;
@@ -575,7 +595,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         live = TMA ? (here & 1u ? 0xffffu : 0u) | (here & 2u ? 0xffff0000u : 0u) : here;
         if (left < kTile) live &= (1u << left) - 1u;
         if (!((live >> lane) & 1u)) {
-          const uint32_t par = st + (lane >> 4) * G::kUnitBytes + (kUnit + (lane & 15)) * G::kRow + HD / 2;
+          const uint32_t par = st + (lane >> 4) * kStage + (kUnit + (lane & 15)) * kStride + HD / 2;
 #pragma unroll
           for (int g = 0; g < NG; ++g) asm volatile("st.shared.b32 [%0], %1;" ::"r"(par + 4 * g), "r"(0) : "memory");
         }
@@ -587,7 +607,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       float s[2][2][NH];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t k0 = st + u * G::kUnitBytes + gid * G::kRow, k1 = k0 + 8 * G::kRow;
+        const uint32_t k0 = st + u * kStage + gid * kStride, k1 = k0 + 8 * kStride;
         float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NZ; ++j) {
@@ -662,7 +682,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          lds(par[u][r], st + u * G::kUnitBytes + (kUnit + gid + 8 * r) * G::kRow + HD / 2);
+          lds(par[u][r], st + u * kStage + (kUnit + gid + 8 * r) * kStride + HD / 2);
 #pragma unroll
           for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -721,7 +741,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          lds(x[u][t], st + u * G::kUnitBytes + (kUnit + 2 * tig + (t & 1) + 8 * (t >> 1)) * G::kRow + gid * NW * 4);
+          lds(x[u][t], st + u * kStage + (kUnit + 2 * tig + (t & 1) + 8 * (t >> 1)) * kStride + gid * NW * 4);
 #pragma unroll
       for (int k = 0; k < NW; ++k) {  // groups 2 k and 2 k + 1
         uint32_t w[2][2][2][4];       // [unit][group][tokens 2 tig.. / 8 further][register]
@@ -762,10 +782,14 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
             }
         }
       }
-      __syncwarp();
+      give_back();
     }
     if constexpr (!TMA) copy_wait<0>();
     __syncwarp();
+    if (given_up) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n) l[n] = __uint_as_float(0x7fc00000u);
+    }
 
 #pragma unroll
     for (int n = 0; n < NH; ++n) m[n] = m[n] == -INFINITY ? m[n] : m[n] * factor[n];
@@ -880,8 +904,9 @@ inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, 
 
 // The pool as a tensor of 8-byte words [block][K / V][token][head][row], boxes of a unit's rows of one head. Where a
 // head's rows of a page are contiguous (head-first pools) and a unit's are no longer than a box may be, the tokens
-// are part of the innermost dimension: 2 runs a box instead of 32.
-inline bool make_map(CUtensorMap* map, const Cache& c, int row, bool* flat) {
+// are part of the innermost dimension: 2 runs a box instead of 32. `shared`, if asked for and the pool is
+// token-first with an even number of heads: a box has the rows of two heads.
+inline bool make_map(CUtensorMap* map, const Cache& c, int row, bool* flat, bool* shared) {
   static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -891,11 +916,14 @@ inline bool make_map(CUtensorMap* map, const Cache& c, int row, bool* flat) {
   }();
   if (!fn || c.num_blocks < 1) return false;
   *flat = c.token_stride == row && kUnit * row / 8 <= 256;
-  const cuuint64_t words = static_cast<cuuint64_t>(row) / 8;
-  const cuuint64_t dims[5] = {*flat ? words * c.page : words, static_cast<cuuint64_t>(c.heads),
+  *shared = *shared && !*flat && c.head_stride == row && c.heads % 2 == 0;
+  const int64_t head_stride = *shared ? 2 * c.head_stride : c.head_stride;
+  const int heads = *shared ? c.heads / 2 : c.heads;
+  const cuuint64_t words = static_cast<cuuint64_t>(row) / 8 * (*shared ? 2 : 1);
+  const cuuint64_t dims[5] = {*flat ? words * c.page : words, static_cast<cuuint64_t>(heads),
                               *flat ? 1 : static_cast<cuuint64_t>(c.page), 2, static_cast<cuuint64_t>(c.num_blocks)};
   // a dimension of one may come with any stride
-  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(c.heads > 1 ? c.head_stride : row),
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(heads > 1 ? head_stride : row),
                                  static_cast<cuuint64_t>(c.token_stride), static_cast<cuuint64_t>(c.outer_stride),
                                  static_cast<cuuint64_t>(c.num_blocks > 1 ? c.block_stride : row)};
   const cuuint32_t box[5] = {static_cast<cuuint32_t>(*flat ? words * kUnit : words), 1,
@@ -922,9 +950,9 @@ cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, int smem, cudaSt
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int HD, bool PAIR, bool TMA>
+template <int HD, bool PAIR, Copies COPIES>
 cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, const Plan& plan, cudaStream_t stream) {
-  auto kernel = kv4_decode_kernel<HD, PAIR, TMA>;
+  auto kernel = kv4_decode_kernel<HD, PAIR, COPIES>;
   const int warps = plan.y_cta * plan.streams;
   constexpr int kVals = (PAIR ? 1 : 2) * (2 + 4 * (HD / kGroup));  // merging streams, in the ring's place
   const int smem = warps * std::max(Geometry<HD>::kRingBytes, kVals * 128);
@@ -936,14 +964,26 @@ cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, co
 template <int HD>
 cudaError_t launch_decode_hd(AttnParams& P, const Plan& plan, cudaStream_t stream) {
   CUtensorMap map{};
-  const bool tma = P.cache.page % kUnit == 0 && make_map(&map, P.cache, row_bytes(HD), &P.flat);
+  bool shared = HD < 256 && plan.chunks == 1 && plan.y_cta % 2 == 0;
+  const bool tma = P.cache.page % kUnit == 0 && make_map(&map, P.cache, row_bytes(HD), &P.flat, &shared);
   cudaError_t e;
-  if (P.group <= 4)
-    e = tma ? launch_decode_kernel<HD, true, true>(P, map, plan, stream)
-            : launch_decode_kernel<HD, true, false>(P, map, plan, stream);
-  else
-    e = tma ? launch_decode_kernel<HD, false, true>(P, map, plan, stream)
-            : launch_decode_kernel<HD, false, false>(P, map, plan, stream);
+  if constexpr (HD == 256) {
+    if (P.group <= 4)
+      e = tma ? launch_decode_kernel<HD, true, kTma>(P, map, plan, stream)
+              : launch_decode_kernel<HD, true, kRows>(P, map, plan, stream);
+    else
+      e = tma ? launch_decode_kernel<HD, false, kTma>(P, map, plan, stream)
+              : launch_decode_kernel<HD, false, kRows>(P, map, plan, stream);
+  } else {
+    if (P.group <= 4)
+      e = !tma     ? launch_decode_kernel<HD, true, kRows>(P, map, plan, stream)
+          : shared ? launch_decode_kernel<HD, true, kTmaShared>(P, map, plan, stream)
+                   : launch_decode_kernel<HD, true, kTma>(P, map, plan, stream);
+    else
+      e = !tma     ? launch_decode_kernel<HD, false, kRows>(P, map, plan, stream)
+          : shared ? launch_decode_kernel<HD, false, kTmaShared>(P, map, plan, stream)
+                   : launch_decode_kernel<HD, false, kTma>(P, map, plan, stream);
+  }
   if (e != cudaSuccess || plan.ctas == 1) return e;
   const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 2 * 148 ? 1 : kMergeWarps;
   return launch_overlapped(kv4_merge_kernel<HD>, dim3((P.hq + heads_cta - 1) / heads_cta, P.batch), kMergeWarps * 32, 0,

@@ -44,9 +44,10 @@
 // 8, several streams of tokens), so that what lies together in a token-first pool
 // is read together. All requests' tiles are laid end to end and cut into equal
 // ranges, one for each CTA the GPU holds at a time, so ragged batches and odd
-// numbers of heads cost no idle SMs. A CTA meets at most two requests that are
-// not its own alone; their partial results (m, l, acc) are merged by a second
-// kernel, whose launch overlaps the first's end.
+// numbers of heads cost no idle SMs; a cut that falls into a short request moves
+// to its end. A CTA meets at most two requests that are not its own alone; their
+// partial results (m, l, acc) are merged by a second kernel, whose launch overlaps
+// the first's end and is left out where the table holds short requests only.
 //
 // Copies. Each warp has its own ring of two tiles. A unit of 16 tokens, K and V
 // rows of one KV head, is one TMA box of the five-dimensional pool, issued by the
@@ -93,6 +94,7 @@ enum Copies { kRows, kTma, kTmaShared };
 constexpr int kUnit = 16;       // tokens a stage of the ring holds
 constexpr int kTile = 32;       // tokens a warp takes between two updates of its accumulators
 constexpr int kMinRounds = 2;   // a CTA takes at least so many tiles a warp: below, merging costs more than it saves
+constexpr int kWhole = 6;       // requests of up to so many rounds (kStart among them) are not cut
 constexpr uint64_t kWaitNs = 1000000000ull;  // after which a warp gives a copy up
 
 __device__ int g_kv4_status = 0;
@@ -331,9 +333,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // ---- this CTA's range of rounds, and the request it begins in
   __shared__ int64_t warp_sum[kMaxWarps];
-  __shared__ int64_t start_first;
-  __shared__ int start_b;
-  int64_t f, f_end, per;
+  __shared__ int64_t cut_at[2], cut_first;
+  __shared__ int cut_b;
+  int64_t per;
   {
     const int each = (P.batch + blockDim.x - 1) / blockDim.x;
     const int b0 = min(P.batch, static_cast<int>(threadIdx.x) * each), b1 = min(P.batch, b0 + each);
@@ -346,6 +348,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       if (lane >= o) run += x;
     }
     if (lane == 31) warp_sum[warp] = run;
+    if (threadIdx.x < 2) cut_at[threadIdx.x] = INT64_MAX;
     __syncthreads();
     int64_t before = run - sum, total = 0;
     for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
@@ -353,24 +356,35 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       total += warp_sum[w];
     }
     per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinRounds));
-    f = blockIdx.x * per;
-    f_end = min(total, f + per);
-    if (f >= total) return;
-    if (before <= f && f < before + sum) {
-      int b = b0;
-      for (; b < b1 - 1; ++b) {
-        const int n = rounds_of(tokens_of(P, b), P.streams);
-        if (f < before + n) break;
-        before += n;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // where this CTA begins, and where the next one does
+      int64_t cut = (blockIdx.x + i) * per, at = before;
+      if (at <= cut && cut < before + sum) {
+        int b = b0, n = rounds_of(tokens_of(P, b), P.streams);
+        while (cut >= at + n) {
+          at += n;
+          n = rounds_of(tokens_of(P, ++b), P.streams);
+        }
+        if (cut > at && n <= kWhole) {  // into a short request: behind it
+          cut = at += n;
+          ++b;
+        }
+        cut_at[i] = cut;
+        if (i == 0) {
+          cut_b = b;
+          cut_first = at;
+        }
       }
-      start_b = b;
-      start_first = before;
     }
     __syncthreads();
+    if (threadIdx.x < 2) cut_at[threadIdx.x] = min(cut_at[threadIdx.x], total);
+    __syncthreads();
   }
-  const int64_t f_begin = f;
-  int b = start_b;
-  int64_t first = start_first;
+  int64_t f = cut_at[0];
+  const int64_t f_begin = f, f_end = cut_at[1];
+  if (f >= f_end) return;
+  int b = cut_b;
+  int64_t first = cut_first;
   const int yw = warp % P.y_cta, stream = warp / P.y_cta;
   const int y = blockIdx.y * P.y_cta + yw;
   const bool active = y < P.y_total;
@@ -868,7 +882,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       }
       if (r_begin == 0 && y == 0 && lane == 0)
         P.parts[b] = make_int2(2 * blockIdx.x + (f == f_begin ? 0 : 1),
-                               static_cast<int>((first + rounds - 1) / per) - static_cast<int>(blockIdx.x) + 1);
+                               whole_request ? 1 : static_cast<int>((first + rounds - 1) / per) - static_cast<int>(blockIdx.x) + 1);
     }
     f = first + r_end;
     if (r_end == rounds) {
@@ -881,24 +895,32 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 // How a launch is laid out: (KV head, chunk) pairs and streams a CTA, CTAs along the work.
 struct Plan {
   int chunks, y_total, y_cta, y_ctas, streams, ctas;
+  bool cut;  // whether a request may be cut, and the merge is to follow
 };
 inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, int ctas, int sm_count) {
   Plan p{};
   p.chunks = (hq / hkv + kHeads - 1) / kHeads;
   p.y_total = hkv * p.chunks;
-  // As many KV heads a CTA as it has warps, unless requests are so few that each would be cut into more than 32
-  // parts: streams of tokens are merged within a CTA, parts by the second kernel (131,072 tokens of one request,
-  // 8 KV heads: 296 parts of 8 heads 69 us, 37 of one head 44 us).
-  for (p.y_cta = (p.y_total + (p.y_total - 1) / kMaxWarps) / ((p.y_total - 1) / kMaxWarps + 1);; --p.y_cta) {
-    p.y_ctas = (p.y_total + p.y_cta - 1) / p.y_cta;
-    p.streams = kMaxWarps / p.y_cta;
-    // registers allow 16 warps an SM (8 with 256 elements a head)
-    const int per_sm = std::max(1, (hd == 256 ? 8 : 16) / (p.y_cta * p.streams));
+  // Where requests are short and few, one KV head a CTA: its 8 streams of tokens take a request's 1,024 tokens in 4
+  // rounds, and nothing is cut (600 tokens of one request, 8 KV heads: 8.8 us in place of 10.5). Else as many as it has warps, an even
+  // number so that pairs can share copies, unless requests are so few that each would be cut into more than 80 parts
+  // (131,072 tokens of one request, 8 KV heads: 296 parts of 8 heads 40 us, 74 of two 37 us, 37 of one 47 us).
+  const int most = (hd == 256 ? 8 : 16) / kMaxWarps;  // registers allow 16 warps an SM (8 with 256 elements a head)
+  const bool short_few = kStart + (max_tokens + 8 * kTile - 1) / (8 * kTile) <= kWhole &&
+                         static_cast<int64_t>(batch) * p.y_total <= 2 * most * sm_count;
+  for (int n = (p.y_total + kMaxWarps - 1) / kMaxWarps;; ++n) {
+    const int y = short_few ? 1 : (p.y_total + n - 1) / n;
+    if (y > 1 && y % 2 != 0 && y < kMaxWarps && p.y_total % 2 == 0) continue;
+    p.y_cta = y;
+    p.y_ctas = (p.y_total + y - 1) / y;
+    p.streams = kMaxWarps / y;
+    const int per_sm = std::max(1, most * kMaxWarps / (y * p.streams));
     p.ctas = ctas > 0 ? ctas : std::max(1, sm_count * per_sm / p.y_ctas);
-    if (p.ctas / batch < 32 || p.y_cta == 1) break;
+    if (p.ctas / batch <= 80 || y <= 2) break;
   }
   const int64_t rounds = (max_tokens + kTile * p.streams - 1) / (kTile * p.streams);
-  p.ctas = static_cast<int>(std::min<int64_t>(p.ctas, std::max<int64_t>(1, (batch * rounds + kMinRounds - 1) / kMinRounds)));
+  p.ctas = static_cast<int>(std::min<int64_t>(p.ctas, std::max<int64_t>(1, (batch * (rounds + kStart) + kMinRounds - 1) / kMinRounds)));
+  p.cut = p.ctas > 1 && rounds + kStart > kWhole;
   return p;
 }
 
@@ -984,7 +1006,7 @@ cudaError_t launch_decode_hd(AttnParams& P, const Plan& plan, cudaStream_t strea
           : shared ? launch_decode_kernel<HD, false, kTmaShared>(P, map, plan, stream)
                    : launch_decode_kernel<HD, false, kTma>(P, map, plan, stream);
   }
-  if (e != cudaSuccess || plan.ctas == 1) return e;
+  if (e != cudaSuccess || !plan.cut) return e;
   const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 2 * 148 ? 1 : kMergeWarps;
   return launch_overlapped(kv4_merge_kernel<HD>, dim3((P.hq + heads_cta - 1) / heads_cta, P.batch), kMergeWarps * 32, 0,
                            stream, P, heads_cta);

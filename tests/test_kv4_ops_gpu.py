@@ -331,6 +331,11 @@ def _check_attn(got, q, vals, scale, **kw):
         ([700, 0, 900, 1], 3, 3, 128, 32, "hnd", 2),              # CTAs that begin and end inside requests
         ([150] * 9, 12, 2, 64, 16, "nhd", 5),                     # more KV heads than a CTA has warps
         ([6000], 5, 4, 128, 16, "nhd", 0),
+        ([20000], 8, 2, 64, 16, "nhd", 0),                        # one request in 74 parts
+        ([60000] + [5, 0, 17] * 13, 1, 8, 64, 16, "nhd", 0),      # a request in many parts among short ones
+        ([700, 30, 1200, 5, 90, 2000] * 5, 4, 4, 128, 16, "nhd", 0),  # cuts that move behind short requests
+        ([64, 100, 31], 6, 2, 64, 32, "nhd", 0),                  # pairs of heads, 6 of them
+        ([640, 100, 3100], 4, 6, 64, 16, "nhd", 0),
 ])
 def test_paged_decode_attention(lens, hkv, group, hd, page, order, ctas):
     B = len(lens)

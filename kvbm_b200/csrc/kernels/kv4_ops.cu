@@ -27,9 +27,13 @@ constexpr int kThreads = 256;
 // A row of HD elements is held by HD/16 lanes, each with 8 elements of the first
 // half and the 8 that lie HD/2 behind them, so with rot = HD both elements of a
 // rotation are in one lane (with a smaller rot the other comes by shuffle), and
-// a warp takes 512 / HD rows a step. With w folded into the cosines and sines
-// once a token, out = 1/rms (x (w cos) - x' (w' sin)) costs three multiplies an
-// element, done in pairs.
+// a warp takes 512 / HD rows a step. Every product is rounded to fp32 by itself in
+// the order of the formula, and the squares are summed in the order of an unfused
+// evaluation (sum_squares), so that k's bf16 values, and with them the codes of a
+// 4-bit cache, do not depend on which of the two computed them: one fp32 step
+// moves a code that lies next to a border by a fifteenth of its group's range
+// (folding w into cos and sin, two of five products less an element, moved 4 codes
+// in a chunk of 8,192 tokens).
 // What bounds it is HBM for a prefill (the rows go in and out once), nearly
 // matched by the instructions of the norm, the rotation and the quantising: hence
 // the packed arithmetic, and the next step's loads in flight under each step. For
@@ -66,6 +70,57 @@ __device__ __forceinline__ void words(uint32_t (&x)[4], int4 v) { x[0] = v.x, x[
 
 enum Kind { kQ, kK, kV };
 
+// Sum of the squares of a row's HD values; this lane has units l and l + HD/16. The order: at 256, the two halves of
+// the row are added element by element first; at 128 and 256, each four neighbours one after another; then the upper
+// half of what is left is added to the lower half until one value is left.
+template <int HD>
+__device__ __forceinline__ float sum_squares(const f32x2 (&y)[2][4]) {
+  float a[8], b[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    kv4::split2(y[0][k], a[2 * k], a[2 * k + 1]);
+    kv4::split2(y[1][k], b[2 * k], b[2 * k + 1]);
+  }
+  // squares of bf16 values are exact in fp32, so a fused multiply-add is a rounded sum of squares
+  if constexpr (HD == 64) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = fmaf(b[k], b[k], a[k] * a[k]);
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] += __shfl_xor_sync(0xffffffffu, a[k], o);
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+      for (int k = 0; k < n; ++k) a[k] += a[k + n];
+    return a[0];
+  } else {
+    float r[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (HD == 128) {
+        float qa = a[4 * i] * a[4 * i], qb = b[4 * i] * b[4 * i];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) {
+          qa = fmaf(a[4 * i + k], a[4 * i + k], qa);
+          qb = fmaf(b[4 * i + k], b[4 * i + k], qb);
+        }
+        r[i] = qa + qb;
+      } else {
+#pragma unroll
+        for (int k = 4 * i; k < 4 * i + 4; ++k) a[k] = fmaf(b[k], b[k], a[k] * a[k]);
+        r[i] = __fadd_rn(__fadd_rn(__fadd_rn(a[4 * i], a[4 * i + 1]), a[4 * i + 2]), a[4 * i + 3]);
+      }
+    }
+#pragma unroll
+    for (int o = HD / 32; o > 0; o >>= 1) {
+      r[0] += __shfl_xor_sync(0xffffffffu, r[0], o);
+      r[1] += __shfl_xor_sync(0xffffffffu, r[1], o);
+    }
+    return r[0] + r[1];
+  }
+}
+
 template <int HD, bool KV4, bool FULL, Kind KIND>
 __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int begin, int end, int32_t pos,
                                            uint8_t* cache_row) {
@@ -85,8 +140,9 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
   };
   load(begin);
 
-  // Unit i of this lane (8 elements): out = x cw[i] + x' sw[i], x' the unit `other[i]` of the row.
-  f32x2 cw[2][4], sw[2][4];
+  // Unit i of this lane (8 elements): with y = x / rms w, out = y cs[i] + y' sn[i], y' the unit `other[i]` of the row.
+  f32x2 cs[2][4], sn[2][4];
+  uint32_t wt[2][4], wt_other[2][4];  // bf16 pairs
   int other[2];
   const __nv_bfloat16* w = KIND == kQ ? P.q_weight : P.k_weight;
   if constexpr (KIND != kV) {
@@ -96,27 +152,21 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
       const int u = l + i * L;
       other[i] = u < half ? u + half : u < 2 * half ? u - half : u;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) cw[i][k] = kv4::make2(1.f, 1.f), sw[i][k] = 0;
+      for (int k = 0; k < 4; ++k) cs[i][k] = kv4::make2(1.f, 1.f), sn[i][k] = 0;
       if (FULL || u < 2 * half) {
-        const float* cs = P.cos_sin + static_cast<int64_t>(pos) * (FULL ? HD : P.rot) + (u < half ? u : u - half) * 8;
+        const float* at = P.cos_sin + static_cast<int64_t>(pos) * (FULL ? HD : P.rot) + (u < half ? u : u - half) * 8;
         const float sign = u < half ? -1.f : 1.f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float4 a = *reinterpret_cast<const float4*>(cs + 4 * k);
-          const float4 b = *reinterpret_cast<const float4*>(cs + 8 * half + 4 * k);
-          cw[i][2 * k] = kv4::make2(a.x, a.y), cw[i][2 * k + 1] = kv4::make2(a.z, a.w);
-          sw[i][2 * k] = kv4::make2(sign * b.x, sign * b.y), sw[i][2 * k + 1] = kv4::make2(sign * b.z, sign * b.w);
+          const float4 a = *reinterpret_cast<const float4*>(at + 4 * k);
+          const float4 b = *reinterpret_cast<const float4*>(at + 8 * half + 4 * k);
+          cs[i][2 * k] = kv4::make2(a.x, a.y), cs[i][2 * k + 1] = kv4::make2(a.z, a.w);
+          sn[i][2 * k] = kv4::make2(sign * b.x, sign * b.y), sn[i][2 * k + 1] = kv4::make2(sign * b.z, sign * b.w);
         }
       }
       if (w != nullptr) {
-        uint32_t wm[4], wp[4];
-        words(wm, reinterpret_cast<const int4*>(w)[u]);
-        words(wp, reinterpret_cast<const int4*>(w)[other[i]]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          cw[i][k] = kv4::mul2(cw[i][k], kv4::widen(wm[k]));
-          sw[i][k] = kv4::mul2(sw[i][k], kv4::widen(wp[k]));
-        }
+        words(wt[i], reinterpret_cast<const int4*>(w)[u]);
+        if constexpr (!FULL) words(wt_other[i], reinterpret_cast<const int4*>(w)[other[i]]);
       }
     }
   }
@@ -127,41 +177,49 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
     words(x[1], next[1]);
     load(step + 1);
     if constexpr (KIND != kV) {
-      f32x2 v[2][4], y[2][4], ss2 = 0;
+      f32x2 y[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[i][k] = kv4::widen(x[i][k]);
-          ss2 = kv4::fma2(v[i][k], v[i][k], ss2);
-        }
+        for (int k = 0; k < 4; ++k) y[i][k] = kv4::widen(x[i][k]);
+      f32x2 p[2][4];
+      if constexpr (!FULL) {  // the other unit lies in lane other % L, as its first or its second
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f32x2 p;
-          if constexpr (FULL) {
-            p = v[1 - i][k];
-          } else {  // the unit lies in lane other % L, as its first or its second
+          for (int k = 0; k < 4; ++k) {
             const uint32_t a = __shfl_sync(0xffffffffu, x[0][k], other[i] % L, L);
             const uint32_t b = __shfl_sync(0xffffffffu, x[1][k], other[i] % L, L);
-            p = kv4::widen(other[i] < L ? a : b);
+            p[i][k] = kv4::widen(other[i] < L ? a : b);
           }
-          y[i][k] = kv4::fma2(v[i][k], cw[i][k], kv4::mul2(p, sw[i][k]));
-        }
+      }
       if (w != nullptr) {
-        float ss, hi;
-        kv4::split2(ss2, ss, hi);
-        ss += hi;
-#pragma unroll
-        for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(fmaf(ss, 1.f / HD, P.eps));
+        const float inv = rsqrtf(fmaf(sum_squares<HD>(y), 1.f / HD, P.eps));
         const f32x2 inv2 = kv4::make2(inv, inv);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[i][k] = kv4::mul2(y[i][k], inv2);
+          for (int k = 0; k < 4; ++k) {
+            y[i][k] = kv4::mul2(kv4::mul2(y[i][k], inv2), kv4::widen(wt[i][k]));
+            if constexpr (!FULL) p[i][k] = kv4::mul2(kv4::mul2(p[i][k], inv2), kv4::widen(wt_other[i][k]));
+          }
       }
+      if constexpr (FULL) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) p[i][k] = y[1 - i][k];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // added one by one: the compiler fuses a packed product and a packed sum
+          float a0, a1, b0, b1;
+          kv4::split2(kv4::mul2(y[i][k], cs[i][k]), a0, a1);
+          kv4::split2(kv4::mul2(p[i][k], sn[i][k]), b0, b1);
+          y[i][k] = kv4::make2(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -204,7 +262,7 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
 }
 
 template <int HD, bool KV4, bool FULL>
-__global__ void __launch_bounds__(kThreads, 3) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
+__global__ void __launch_bounds__(kThreads, FULL ? 3 : 2) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (item >= P.tokens * P.items_div.d) return;
   const int64_t t = P.items_div.div(static_cast<uint32_t>(item));

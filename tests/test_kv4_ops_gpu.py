@@ -545,3 +545,44 @@ def test_operators_together_captured_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def _unfused(x, w, cos_sin, rot, eps):
+    """The formula in fp32, each operation rounded by itself, the squares summed in the kernel's order."""
+    y = x.float()
+    s = y * y
+    if s.shape[-1] == 256:
+        s = s[..., :128] + s[..., 128:]
+    if x.shape[-1] > 64:
+        s = s.unflatten(-1, (32, 4))
+        s = ((s[..., 0] + s[..., 1]) + s[..., 2]) + s[..., 3]
+    while s.shape[-1] > 1:
+        n = s.shape[-1] // 2
+        s = s[..., :n] + s[..., n:]
+    y = y * torch.rsqrt(s / x.shape[-1] + eps) * w.float()
+    c, n = cos_sin[:, None, :rot // 2], cos_sin[:, None, rot // 2:]
+    a, b = y[..., :rot // 2], y[..., rot // 2:rot]
+    return torch.cat([a * c - b * n, b * c + a * n, y[..., rot:]], -1).bfloat16()
+
+
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 16), (128, 128), (128, 48), (256, 256), (256, 64)])
+def test_write_rounds_as_the_unfused_formula(hd, rot):
+    """k decides the codes of the cache, so it is the same bit for bit as each operation by itself."""
+    tokens, hq, hkv, page = 193, 6, 3, 16
+    gen = torch.Generator().manual_seed(hd + rot)
+    qkv = torch.randn(tokens, hq + 2 * hkv, hd, generator=gen).bfloat16().cuda()
+    wq, wk = ((1 + 0.2 * torch.randn(hd, generator=gen)).bfloat16().cuda() for _ in range(2))
+    angle = 6.0 * torch.rand(tokens, rot // 2, generator=gen)
+    cos_sin = torch.cat([angle.cos(), angle.sin()], -1).cuda()
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    slots = torch.arange(tokens, device="cuda")
+    kv = torch.zeros(13, 2, page, hkv, kv4_ops.row_bytes(hd), dtype=torch.uint8, device="cuda")
+    q = torch.empty(tokens, hq, hd, dtype=torch.bfloat16, device="cuda")
+    k = torch.empty(tokens, hkv, hd, dtype=torch.bfloat16, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(qkv, positions, cos_sin, hq, hkv, kv, slots, q_weight=wq, k_weight=wk, eps=1e-6,
+                                  q_out=q, k_out=k)
+    assert torch.equal(q, _unfused(qkv[:, :hq], wq, cos_sin, rot, 1e-6))
+    want = _unfused(qkv[:, hq:hq + hkv], wk, cos_sin, rot, 1e-6)
+    assert torch.equal(k, want)
+    rows = kv[:, 0].reshape(-1, hkv, kv4_ops.row_bytes(hd))[:tokens].cpu()
+    assert torch.equal(rows, kv4_ops.pack_rows(want.cpu(), False))

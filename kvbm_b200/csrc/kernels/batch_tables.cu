@@ -165,8 +165,6 @@ __global__ void __launch_bounds__(kThreads) slot_map_kernel(const int32_t* __res
 
 }  // namespace
 
-extern "C" int kvbm_batch_tables_max_batch(void) { return kMaxBatch; }
-
 extern "C" int kvbm_batch_tables(const int32_t* query_lens, const int32_t* context_lens, const int32_t* block_counts,
                                  const int32_t* block_ids, int64_t num_ids, int batch, int page, int max_blocks,
                                  int pad, int32_t* table, int64_t table_stride, const int32_t* rows, int num_rows,

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const __grid_const
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 bool cache_ok(const Cache& c) {
-  return c.base != nullptr && aligned16(c.base) && c.block_stride % 16 == 0 && c.outer_stride % 16 == 0 &&
+  return (c.base != nullptr || c.num_blocks == 0) && aligned16(c.base) && c.block_stride % 16 == 0 && c.outer_stride % 16 == 0 &&
          c.token_stride % 16 == 0 && c.head_stride % 16 == 0 && c.page > 0 && c.num_blocks >= 0 && c.heads > 0;
 }
 

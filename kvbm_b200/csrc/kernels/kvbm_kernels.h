@@ -211,7 +211,6 @@ int kvbm_batch_tables(const int32_t* query_lens, const int32_t* context_lens, co
                       const int32_t* block_ids, int64_t num_ids, int batch, int page, int max_blocks, int pad,
                       int32_t* table, int64_t table_stride, const int32_t* rows, int num_rows, int32_t* seq_lens,
                       int32_t* cu_query, int32_t* positions, int64_t* slots, int64_t tokens, cudaStream_t stream);
-int kvbm_batch_tables_max_batch(void);
 int kvbm_slot_map(const int32_t* table, int64_t row_stride, int max_blocks, const int32_t* positions, int64_t tokens,
                   int page, int64_t* slots, cudaStream_t stream);
 

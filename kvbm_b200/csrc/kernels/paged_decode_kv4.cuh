@@ -855,6 +855,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           }
         }
       }
+      if constexpr (TMA) fence_proxy_async_smem();  // the next request's copies come behind
       __syncthreads();
     }
     // ---- to the output, or to this CTA's slot of partial results

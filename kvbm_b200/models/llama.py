@@ -210,6 +210,7 @@ class LlamaModel:
         self.cos_sin = torch.cat([f.cos(), f.sin()], dim=-1).float().to(self.device)
         self.scale = 1.0 / math.sqrt(c.head_dim)
         self._decode_scratch: torch.Tensor | None = None
+        self._outgrown: list = []
         self._decode_counters: torch.Tensor | None = None
         self.decode_gemm = "cublas"  # "tc": decode projections on the tcgen05 skinny GEMM
         self._gemm_ws: llama_ops.GemmWorkspace | None = None
@@ -362,6 +363,7 @@ class LlamaModel:
 
     def _scratch(self, need: int) -> torch.Tensor:
         if self._decode_scratch is None or self._decode_scratch.numel() < need:
+            self._outgrown.append(self._decode_scratch)  # a captured step goes on using it
             self._decode_scratch = torch.empty(need, dtype=torch.float32, device=self.device)
         return self._decode_scratch
 
@@ -392,6 +394,7 @@ class LlamaModel:
         c = self.cfg
         B = tokens.numel()
         page = pool.config.page_size
+        block_table = block_table[:B]
         slots = table_ops.slot_map(block_table, positions, page=page)
         x = F.embedding(tokens, self.embed)
         residual = x

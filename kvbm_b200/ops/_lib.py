@@ -131,7 +131,6 @@ _SIGS = {
         _INT,
         [_VP, _VP, _VP, _VP, _I64, _INT, _INT, _INT, _INT, _VP, _I64, _VP, _INT, _VP, _VP, _VP, _VP, _I64, _VP],
     ),
-    "kvbm_batch_tables_max_batch": (_INT, []),
     "kvbm_slot_map": (_INT, [_VP, _I64, _INT, _VP, _I64, _INT, _VP, _VP]),
     "kvbm_qk_norm_rope_kv_write": (
         _INT,

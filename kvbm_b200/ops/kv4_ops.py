@@ -100,6 +100,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: t
     token_stride, head_stride, unit = qkv.stride()
     if unit != 1 or (H > 1 and head_stride != hd) or (T > 1 and token_stride & 7) or qkv.data_ptr() & 15:
         raise ValueError("qkv needs contiguous heads and 16-byte aligned tokens")
+    if T > 1 and token_stride < H * hd and q_out is None:
+        raise ValueError("tokens of qkv that overlap cannot be rotated in place")
     bits = 16 if kv.dtype == torch.bfloat16 else 4
     cache, heads, row = _cache_args(kv, dev, bits)
     if heads != hkv or row != (hd if bits == 16 else row_bytes(hd)):
@@ -118,6 +120,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: t
     qw = _weight(q_weight, "q_weight", hd, dev)
     kw = _weight(k_weight, "k_weight", hd, dev)
     qo = _rows_out(q_out, "q_out", (T, hq, hd), dev)
+    if q_out is not None and hq == 0:
+        qo = qkv.data_ptr()  # an empty tensor has no address, and none would mean in place: nothing is written there
     ko = _rows_out(k_out, "k_out", (T, hkv, hd), dev)
     with _lib.on_device(dev, stream) as st:
         _lib.call("kvbm_qk_norm_rope_kv_write", qkv.data_ptr(), token_stride, T, hq, hkv, hd, rot,
@@ -221,7 +225,7 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
 
 def kv4_status(reset: bool = True) -> int:
     """0, or the error a :func:`paged_decode_attn_kv4` launch recorded (3: a wait for a copy timed out; its results
-    are NaN). Synchronizes."""
+    are NaN) on the current device. Synchronizes."""
     return int(_lib.load().kvbm_kv4_status(1 if reset else 0))
 
 

@@ -136,6 +136,40 @@ def test_model_over_a_4_bit_pool(norm, order):
     _near(v4[0], b[1], _behind_attention(b[1]))
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+def test_decode_steps_of_several_sizes(bits):
+    """A captured step keeps its scratch when a larger step needs more; a table may have more rows than the batch."""
+    model = LlamaModel(_cfg(), "cuda", seed=8)
+    pool = model.allocate_pool(128, kv_bits=bits)
+    g = torch.Generator("cuda").manual_seed(4)
+    prompt = torch.randint(0, 1024, (300,), device="cuda", dtype=torch.int32, generator=g)
+    ids = torch.arange(32, dtype=torch.int32, device="cuda")
+    model.prefill(prompt, pool, ids)
+    table = ids.repeat(40, 1)
+    tok, pos = torch.full((1,), 7, device="cuda"), torch.full((1,), 299, dtype=torch.int32, device="cuda")
+
+    def step(B, rows):
+        return model.decode_step(tok.expand(B).contiguous(), pos.expand(B).contiguous(), pool, table[:rows],
+                                 pos.expand(B) + 1, splits=4)
+
+    eager = step(1, 1)
+    assert torch.equal(step(1, 40), eager)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        step(1, 1)
+        with torch.cuda.graph(graph, stream=side):
+            got = step(1, 1)
+    torch.cuda.current_stream().wait_stream(side)
+    small = model._decode_scratch
+    step(40, 40)
+    assert model._decode_scratch.numel() > small.numel() and any(s is small for s in model._outgrown)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, eager)
+
+
 def test_4_bit_pools_refuse_what_they_cannot_do():
     model = LlamaModel(_cfg(), "cuda", seed=1)
     p4, p16 = model.allocate_pool(4, kv_bits=4), model.allocate_pool(4)

@@ -77,6 +77,7 @@ def _write_args(T=3, hq=4, hkv=2, hd=128, **kw):
     (dict(hq=5), "8 heads"),
     (dict(hd=96), "head_dim"),
     (dict(qkv=torch.zeros(3, 128, 8, dtype=BF).transpose(1, 2)), "contiguous heads"),
+    (dict(qkv=torch.zeros(1, 8, 128, dtype=BF).expand(3, 8, 128)), "overlap"),
     (dict(kv=_pool(row=48)), "cache holds"),
     (dict(kv=_pool(heads=1)), "cache holds"),
     (dict(kv=_pool(row=128, dtype=torch.float16)), "4-bit cache"),

@@ -586,3 +586,36 @@ def test_write_rounds_as_the_unfused_formula(hd, rot):
     assert torch.equal(k, want)
     rows = kv[:, 0].reshape(-1, hkv, kv4_ops.row_bytes(hd))[:tokens].cpu()
     assert torch.equal(rows, kv4_ops.pack_rows(want.cpu(), False))
+
+
+def test_write_without_query_heads():
+    """K and V alone: with a q_out of no heads qkv stays as it is."""
+    gen = _gen(11)
+    qkv = torch.randn(5, 4, 128, device="cuda", generator=gen).bfloat16()
+    before = qkv.clone()
+    cos_sin = torch.cat([torch.full((8, 64), 0.6, device="cuda"), torch.full((8, 64), 0.8, device="cuda")], -1)
+    positions = torch.arange(5, dtype=torch.int32, device="cuda")
+    slots = torch.arange(5, device="cuda")
+    kv = _empty_pool(1, 16, 2, 128)
+    k = torch.empty(5, 2, 128, dtype=BF, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(qkv, positions, cos_sin, 0, 2, kv, slots, k_out=k,
+                                  q_out=torch.empty(5, 0, 128, dtype=BF, device="cuda"))
+    assert torch.equal(qkv, before)
+    kv4_ops.qk_norm_rope_kv_write(qkv, positions, cos_sin, 0, 2, _empty_pool(1, 16, 2, 128), slots)
+    assert torch.equal(qkv[:, :2], k) and torch.equal(qkv[:, 2:], before[:, 2:])
+    assert torch.equal(kv[0, 0, :5], kv4_ops.pack_rows(k, False))
+    assert torch.equal(kv[0, 1, :5], kv4_ops.pack_rows(before[:, 2:], True))
+
+
+def test_a_pool_without_blocks():
+    """Nothing is written, rows are zeros, attention has no tokens."""
+    kv = _empty_pool(0, 16, 2, 128)
+    qkv = torch.randn(3, 8, 128, device="cuda", generator=_gen(12)).bfloat16()
+    slots = torch.tensor([0, -1, 7], device="cuda")
+    cos_sin = torch.ones(4, 128, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(qkv, torch.arange(3, dtype=torch.int32, device="cuda"), cos_sin, 4, 2, kv, slots)
+    k, v = kv4_ops.kv4_gather(kv, slots)
+    assert not k.any() and not v.any()
+    out = kv4_ops.paged_decode_attn_kv4(qkv[:, :4], kv, torch.zeros(3, 2, dtype=torch.int32, device="cuda"),
+                                        torch.full((3,), 20, dtype=torch.int32, device="cuda"), 0.1)
+    assert not out.any()

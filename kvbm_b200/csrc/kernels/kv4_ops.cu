@@ -440,12 +440,12 @@ extern "C" int kvbm_paged_decode_attn_kv4_plan(int batch, int hq, int hkv, int h
   if (!out || batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || max_tokens < 0 || ctas < 0 || sm_count <= 0)
     return cudaErrorInvalidValue;
   const kv4::Plan p = kv4::plan_decode(batch, hq, hkv, hd, max_tokens, ctas, sm_count);
-  out[0] = static_cast<int64_t>(p.ctas) * 2 * hq * (hd + 2) + 2 * static_cast<int64_t>(batch);
+  out[0] = p.cut ? static_cast<int64_t>(p.ctas) * 2 * hq * (hd + 2) + 2 * static_cast<int64_t>(batch) : 0;
   out[1] = p.ctas;
   return cudaSuccess;
 }
 
-// `scratch`: 16-byte aligned floats as the plan says.
+// `scratch`: 16-byte aligned floats as the plan says, null for none.
 extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const void* kv, int64_t block_stride,
                                           int64_t outer_stride, int64_t token_stride, int64_t head_stride, int page,
                                           int num_blocks, const int32_t* block_table, int64_t table_stride,
@@ -458,11 +458,11 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
                   page, num_blocks, hkv, FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (batch < 0 || batch > 65535 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || !cache_ok(P.cache) || !q || !aligned16(q) ||
       q_stride % 8 != 0 || !out || !aligned16(out) || !seq_lens || max_blocks < 0 || (max_blocks > 0 && !block_table) ||
-      ctas < 0 || sm_count <= 0 || !scratch || !aligned16(scratch))
+      ctas < 0 || sm_count <= 0 || !aligned16(scratch))
     return cudaErrorInvalidValue;
   const kv4::Plan plan =
       kv4::plan_decode(batch, hq, hkv, hd, static_cast<int64_t>(max_blocks) * page, ctas, sm_count);
-  if (plan.y_ctas > 65535 || static_cast<int64_t>(batch) * hq > 0x7fffffff) return cudaErrorInvalidValue;
+  if (plan.y_ctas > 65535 || static_cast<int64_t>(batch) * hq > 0x7fffffff || (plan.cut && !scratch)) return cudaErrorInvalidValue;
   P.q = static_cast<const __nv_bfloat16*>(q);
   P.q_stride = q_stride;
   P.table = block_table;
@@ -478,9 +478,11 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
   P.streams = plan.streams;
   P.qscale = softmax_scale * 1.4426950408889634f;  // log2(e)
   const int64_t rows = static_cast<int64_t>(plan.ctas) * 2 * hq;
-  P.part_acc = scratch;
-  P.part_ml = scratch + rows * hd;
-  P.parts = reinterpret_cast<int2*>(scratch + rows * (hd + 2));
+  if (plan.cut) {
+    P.part_acc = scratch;
+    P.part_ml = scratch + rows * hd;
+    P.parts = reinterpret_cast<int2*>(scratch + rows * (hd + 2));
+  }
   P.out = static_cast<__nv_bfloat16*>(out);
   return kv4::launch_decode(P, hd, plan, stream);
 }

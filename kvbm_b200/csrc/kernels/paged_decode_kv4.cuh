@@ -83,7 +83,7 @@ struct AttnParams {
   float qscale;
   float* part_acc;  // [cta][2][hq][HD]
   float* part_ml;   // [cta][2][hq][2]
-  int2* parts;      // [batch]: a request's first slot of partial results (2 cta, + 1: not its CTA's first), and how many
+  int2* parts;      // [batch], null if no request can be cut: a request's first slot of partial results (2 cta, + 1: not its CTA's first), and how many
   __nv_bfloat16* out;
   bool flat;  // a head's rows in a page are contiguous: the copies take them as one
 };
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           P.part_ml[(slot_row + h) * 2 + 1] = l[n];
         }
       }
-      if (r_begin == 0 && y == 0 && lane == 0)
+      if (P.parts != nullptr && r_begin == 0 && y == 0 && lane == 0)
         P.parts[b] = make_int2(2 * blockIdx.x + (f == f_begin ? 0 : 1),
                                whole_request ? 1 : static_cast<int>((first + rounds - 1) / per) - static_cast<int>(blockIdx.x) + 1);
     }

@@ -22,13 +22,14 @@ from . import _lib
 
 GROUP = 32
 _HEAD_DIM = {48: 64, 80: 128, 160: 256}  # by row bytes
+_ROW_BYTES = {hd: row for row, hd in _HEAD_DIM.items()}
 
 
 def row_bytes(head_dim: int) -> int:
     """Bytes of one K or V row of ``head_dim`` (64, 128 or 256) elements in 4 bits."""
-    for row, hd in _HEAD_DIM.items():
-        if hd == head_dim:
-            return row
+    row = _ROW_BYTES.get(head_dim)
+    if row is not None:
+        return row
     raise ValueError(f"a 4-bit cache takes head_dim 64, 128 or 256, not {head_dim}")
 
 
@@ -164,7 +165,7 @@ def _decode_plan(batch: int, hq: int, hkv: int, hd: int, max_tokens: int, ctas: 
 def kv4_decode_scratch(batch: int, hq: int, hkv: int, head_dim: int, max_tokens: int, ctas: int = 0,
                        device=None) -> int:
     """Floats of scratch that :func:`paged_decode_attn_kv4` takes for these sizes (``max_tokens``: the block
-    table's width in tokens)."""
+    table's width in tokens); 0 where requests are too short to be cut."""
     dev = torch.device(device if device is not None else "cuda")
     return _decode_plan(batch, hq, hkv, head_dim, max_tokens, ctas,
                         dev.index if dev.index is not None else torch.cuda.current_device())[0]
@@ -214,12 +215,13 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
             return out
         need, sms = _decode_plan(B, hq, hkv, hd, max_blocks * kv.shape[2], ctas, dev.index)
         if scratch is None:
-            scratch = torch.empty(need, dtype=torch.float32, device=dev)
+            if need > 0:
+                scratch = torch.empty(need, dtype=torch.float32, device=dev)
         elif scratch.numel() < need:
             raise ValueError(f"scratch holds {scratch.numel()} floats, {need} are needed")
         _lib.call("kvbm_paged_decode_attn_kv4", q.data_ptr(), row_stride, *cache, block_table.data_ptr() or None,
                   block_table.stride(0), max_blocks, seq_lens.data_ptr(), B, hq, hkv, hd, softmax_scale, ctas, sms,
-                  scratch.data_ptr(), out.data_ptr(), st)
+                  scratch.data_ptr() if need > 0 else None, out.data_ptr(), st)
     return out
 
 

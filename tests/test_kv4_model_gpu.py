@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.nn.functional as F
 
 pytestmark = pytest.mark.gpu
 
@@ -145,7 +146,7 @@ def test_decode_steps_of_several_sizes(bits):
     prompt = torch.randint(0, 1024, (300,), device="cuda", dtype=torch.int32, generator=g)
     ids = torch.arange(32, dtype=torch.int32, device="cuda")
     model.prefill(prompt, pool, ids)
-    table = ids.repeat(40, 1)
+    table = F.pad(ids, (0, 224)).repeat(40, 1)  # wide enough for requests that are cut
     tok, pos = torch.full((1,), 7, device="cuda"), torch.full((1,), 299, dtype=torch.int32, device="cuda")
 
     def step(B, rows):

@@ -619,3 +619,16 @@ def test_a_pool_without_blocks():
     out = kv4_ops.paged_decode_attn_kv4(qkv[:, :4], kv, torch.zeros(3, 2, dtype=torch.int32, device="cuda"),
                                         torch.full((3,), 20, dtype=torch.int32, device="cuda"), 0.1)
     assert not out.any()
+
+
+def test_attention_scratch_of_requests_that_are_cut():
+    lens, hkv, hd, page = [3000, 5, 0, 700], 2, 128, 16
+    kv, table, vals = _filled(4, lens, hkv, hd, page, seed=6)
+    q = torch.randn(4, 8, hd, device="cuda", generator=_gen(2)).to(BF)
+    need = kv4_ops.kv4_decode_scratch(4, 8, hkv, hd, table.shape[1] * page)
+    assert need > 0 and kv4_ops.kv4_decode_scratch(4, 8, hkv, hd, 64) == 0
+    for fill in (math.nan, 3e38):
+        scratch = torch.full((need,), fill, device="cuda")
+        _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, scratch=scratch), q, vals, 0.1)
+    with pytest.raises(ValueError, match="are needed"):
+        kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, scratch=scratch[4:])

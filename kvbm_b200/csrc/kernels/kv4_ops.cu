@@ -56,94 +56,127 @@ struct WriteParams {
   FastDiv items_div;                  // divides by the items of a token
   __nv_bfloat16* q_out;
   __nv_bfloat16* k_out;
+  f32x2 one, minus_one;  // pairs of them
 };
 
-// Read once, possibly written in place later: past L1, but not by the read-only path.
-__device__ __forceinline__ int4 load_once(const void* p) {
-  int4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 __device__ __forceinline__ void words(uint32_t (&x)[4], int4 v) { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+// A unit's 8 bf16 values in fp32, elements k and k + 4 a pair, and back.
+__device__ __forceinline__ void widen8(f32x2 (&y)[4], const uint32_t (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    y[2 * k] = kv4::make2(kv4::bf_lo(x[k]), kv4::bf_lo(x[k + 2]));
+    y[2 * k + 1] = kv4::make2(kv4::bf_hi(x[k]), kv4::bf_hi(x[k + 2]));
+  }
+}
+__device__ __forceinline__ void narrow8(uint32_t (&x)[4], const f32x2 (&y)[4]) {
+  float lo[4], hi[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) kv4::split2(y[k], lo[k], hi[k]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    x[k] = kv4::pack2(lo[2 * k], lo[2 * k + 1]);
+    x[k + 2] = kv4::pack2(hi[2 * k], hi[2 * k + 1]);
+  }
+}
 
 enum Kind { kQ, kK, kV };
 
 // Sum of the squares of a row's HD values; this lane has units l and l + HD/16. The order: at 256, the two halves of
 // the row are added element by element first; at 128 and 256, each four neighbours one after another; then the upper
-// half of what is left is added to the lower half until one value is left.
+// half of what is left is added to the lower half until one value is left. Squares of bf16 values are exact in fp32,
+// so a fused multiply-add is a rounded sum of squares.
 template <int HD>
-__device__ __forceinline__ float sum_squares(const f32x2 (&y)[2][4]) {
-  float a[8], b[8];
+__device__ __forceinline__ float sum_squares(const f32x2 (&a)[4], const f32x2 (&b)[4]) {
+  f32x2 h[4];
+  constexpr int kLeft = HD == 64 ? 4 : 1;  // pairs a lane has left before lanes are added
+  if constexpr (HD == 128) {
+    f32x2 qb = kv4::mul2(b[0], b[0]);
+    h[0] = kv4::mul2(a[0], a[0]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    kv4::split2(y[0][k], a[2 * k], a[2 * k + 1]);
-    kv4::split2(y[1][k], b[2 * k], b[2 * k + 1]);
-  }
-  // squares of bf16 values are exact in fp32, so a fused multiply-add is a rounded sum of squares
-  if constexpr (HD == 64) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = fmaf(b[k], b[k], a[k] * a[k]);
-#pragma unroll
-    for (int o = 2; o > 0; o >>= 1)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) a[k] += __shfl_xor_sync(0xffffffffu, a[k], o);
-#pragma unroll
-    for (int n = 4; n > 0; n >>= 1)
-#pragma unroll
-      for (int k = 0; k < n; ++k) a[k] += a[k + n];
-    return a[0];
+    for (int k = 1; k < 4; ++k) {
+      h[0] = kv4::fma2(a[k], a[k], h[0]);
+      qb = kv4::fma2(b[k], b[k], qb);
+    }
+    h[0] = kv4::add2(h[0], qb);
   } else {
-    float r[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (HD == 128) {
-        float qa = a[4 * i] * a[4 * i], qb = b[4 * i] * b[4 * i];
-#pragma unroll
-        for (int k = 1; k < 4; ++k) {
-          qa = fmaf(a[4 * i + k], a[4 * i + k], qa);
-          qb = fmaf(b[4 * i + k], b[4 * i + k], qb);
-        }
-        r[i] = qa + qb;
-      } else {
-#pragma unroll
-        for (int k = 4 * i; k < 4 * i + 4; ++k) a[k] = fmaf(b[k], b[k], a[k] * a[k]);
-        r[i] = __fadd_rn(__fadd_rn(__fadd_rn(a[4 * i], a[4 * i + 1]), a[4 * i + 2]), a[4 * i + 3]);
-      }
-    }
-#pragma unroll
-    for (int o = HD / 32; o > 0; o >>= 1) {
-      r[0] += __shfl_xor_sync(0xffffffffu, r[0], o);
-      r[1] += __shfl_xor_sync(0xffffffffu, r[1], o);
-    }
-    return r[0] + r[1];
+    for (int k = 0; k < 4; ++k) h[k] = kv4::fma2(b[k], b[k], kv4::mul2(a[k], a[k]));
+    if constexpr (HD == 256) h[0] = kv4::add2(kv4::add2(kv4::add2(h[0], h[1]), h[2]), h[3]);
   }
+#pragma unroll
+  for (int o = HD / 32; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < kLeft; ++k) {
+      float lo, hi;
+      kv4::split2(h[k], lo, hi);
+      h[k] = kv4::add2(h[k], kv4::make2(__shfl_xor_sync(0xffffffffu, lo, o), __shfl_xor_sync(0xffffffffu, hi, o)));
+    }
+  float s[kLeft];
+#pragma unroll
+  for (int k = 0; k < kLeft; ++k) {
+    float lo, hi;
+    kv4::split2(h[k], lo, hi);
+    s[k] = lo + hi;
+  }
+#pragma unroll
+  for (int n = kLeft / 2; n > 0; n >>= 1)
+#pragma unroll
+    for (int k = 0; k < n; ++k) s[k] += s[k + n];
+  return s[0];
 }
 
+// Where a warp's steps find their rows: copies of the next kRing - 1 steps are in flight, across the borders of the
+// kinds too. A lane reads what it copied itself.
+constexpr int kRing = 4;
+struct Rows {
+  const WriteParams& P;
+  const __nv_bfloat16* token;
+  int4* ring;  // this lane's first piece; [kRing][2][32]
+  int end;
+  template <int HD>
+  __device__ __forceinline__ void load(int step) const {
+    constexpr int L = HD / 16, R = 32 / L;
+    const int lane = threadIdx.x & 31, l = lane % L, r = lane / L;
+    if (step < end) {
+      int first = 0, rows = P.hq, at = step;
+      if (at >= P.steps_q) {
+        at -= P.steps_q, first = P.hq, rows = P.hkv;
+        if (at >= P.steps_kv) at -= P.steps_kv, first += P.hkv;
+      }
+      const int h = at * R + r;
+      if (h < rows) {
+        const __nv_bfloat16* src = token + static_cast<int64_t>(first + h) * HD + 8 * l;
+        int4* dst = ring + (step % kRing) * 64;
+        kv4::copy16(smem_u32(dst), src);
+        kv4::copy16(smem_u32(dst + 32), src + HD / 2);
+      }
+    }
+    kv4::copy_commit();
+  }
+  template <int HD>
+  __device__ __forceinline__ void take(int step, uint32_t (&x)[2][4]) const {
+    load<HD>(step + kRing - 1);
+    kv4::copy_wait<kRing - 1>();
+    words(x[0], ring[(step % kRing) * 64]);
+    words(x[1], ring[(step % kRing) * 64 + 32]);
+  }
+};
+
 template <int HD, bool KV4, bool FULL, Kind KIND>
-__device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int begin, int end, int32_t pos,
-                                           uint8_t* cache_row) {
+__device__ __forceinline__ void write_rows(const WriteParams& P, const Rows& from, int64_t t, int first, int begin,
+                                           int end, int32_t pos, uint8_t* cache_row) {
   constexpr int L = HD / 16, R = 32 / L;  // lanes a row, rows a step
   const int lane = threadIdx.x & 31, l = lane % L, r = lane / L;
   const int rows = KIND == kQ ? P.hq : P.hkv;
-  const int head0 = KIND == kQ ? 0 : KIND == kK ? P.hq : P.hq + P.hkv;
-  __nv_bfloat16* src = P.qkv + t * P.qkv_stride + static_cast<int64_t>(head0) * HD + 8 * l;
-  int4 next[2];  // the next step's rows, in flight (two steps ahead cost registers: 24 warps an SM are worth more)
-  auto load = [&](int step) {
-    const int h = step * R + r;
-    next[0] = next[1] = make_int4(0, 0, 0, 0);
-    if (step < end && h < rows) {
-      next[0] = load_once(src + static_cast<int64_t>(h) * HD);
-      next[1] = load_once(src + static_cast<int64_t>(h) * HD + HD / 2);
-    }
-  };
-  load(begin);
 
-  // Unit i of this lane (8 elements): with y = x / rms w, out = y cs[i] + y' sn[i], y' the unit `other[i]` of the row.
-  f32x2 cs[2][4], sn[2][4];
+  // With y = x / rms w and, for unit i of this lane, y' the unit `other[i]` of the row: out = y cs[i] + y' sn[i]. With
+  // all elements rotated the other unit is the lane's own, and cos and sin are the same for both: out[0] = y[0] cs[0]
+  // - y[1] sn[0], out[1] = y[1] cs[0] + y[0] sn[0].
+  constexpr int U = FULL ? 1 : 2;
+  f32x2 cs[U][4], sn[U][4];
   uint32_t wt[2][4], wt_other[2][4];  // bf16 pairs
   int other[2];
+  bool turned[2];
   const __nv_bfloat16* w = KIND == kQ ? P.q_weight : P.k_weight;
   if constexpr (KIND != kV) {
     const int half = FULL ? L : P.rot / 16;  // units that hold one half of the rotated elements
@@ -151,17 +184,19 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
     for (int i = 0; i < 2; ++i) {
       const int u = l + i * L;
       other[i] = u < half ? u + half : u < 2 * half ? u - half : u;
+      turned[i] = u < 2 * half;
+      if (i < U) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) cs[i][k] = kv4::make2(1.f, 1.f), sn[i][k] = 0;
-      if (FULL || u < 2 * half) {
-        const float* at = P.cos_sin + static_cast<int64_t>(pos) * (FULL ? HD : P.rot) + (u < half ? u : u - half) * 8;
-        const float sign = u < half ? -1.f : 1.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float4 a = *reinterpret_cast<const float4*>(at + 4 * k);
-          const float4 b = *reinterpret_cast<const float4*>(at + 8 * half + 4 * k);
-          cs[i][2 * k] = kv4::make2(a.x, a.y), cs[i][2 * k + 1] = kv4::make2(a.z, a.w);
-          sn[i][2 * k] = kv4::make2(sign * b.x, sign * b.y), sn[i][2 * k + 1] = kv4::make2(sign * b.z, sign * b.w);
+        for (int k = 0; k < 4; ++k) cs[i][k] = sn[i][k] = 0;
+        if (FULL || turned[i]) {
+          const float* at = P.cos_sin + static_cast<int64_t>(pos) * (FULL ? HD : P.rot) + (u < half ? u : u - half) * 8;
+          const float sign = FULL || u >= half ? 1.f : -1.f;
+          const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
+          const float4 c = reinterpret_cast<const float4*>(at + 8 * half)[0], d = reinterpret_cast<const float4*>(at + 8 * half)[1];
+          cs[i][0] = kv4::make2(a.x, b.x), cs[i][1] = kv4::make2(a.y, b.y);
+          cs[i][2] = kv4::make2(a.z, b.z), cs[i][3] = kv4::make2(a.w, b.w);
+          sn[i][0] = kv4::make2(sign * c.x, sign * d.x), sn[i][1] = kv4::make2(sign * c.y, sign * d.y);
+          sn[i][2] = kv4::make2(sign * c.z, sign * d.z), sn[i][3] = kv4::make2(sign * c.w, sign * d.w);
         }
       }
       if (w != nullptr) {
@@ -173,60 +208,60 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
   for (int step = begin; step < end; ++step) {
     const int h = step * R + r;
     uint32_t x[2][4];
-    words(x[0], next[0]);
-    words(x[1], next[1]);
-    load(step + 1);
+    from.take<HD>(first + step, x);
     if constexpr (KIND != kV) {
-      f32x2 y[2][4];
+      f32x2 y[2][4], p[2][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) y[i][k] = kv4::widen(x[i][k]);
-      f32x2 p[2][4];
-      if constexpr (!FULL) {  // the other unit lies in lane other % L, as its first or its second
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
+        widen8(y[i], x[i]);
+        if constexpr (!FULL) {  // the other unit lies in lane other % L, as its first or its second
+          uint32_t theirs[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t a = __shfl_sync(0xffffffffu, x[0][k], other[i] % L, L);
             const uint32_t b = __shfl_sync(0xffffffffu, x[1][k], other[i] % L, L);
-            p[i][k] = kv4::widen(other[i] < L ? a : b);
+            theirs[k] = other[i] < L ? a : b;
           }
+          widen8(p[i], theirs);
+        }
       }
       if (w != nullptr) {
-        const float inv = rsqrtf(fmaf(sum_squares<HD>(y), 1.f / HD, P.eps));
+        const float inv = rsqrtf(fmaf(sum_squares<HD>(y[0], y[1]), 1.f / HD, P.eps));
         const f32x2 inv2 = kv4::make2(inv, inv);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+          f32x2 wide[4];
+          widen8(wide, wt[i]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            y[i][k] = kv4::mul2(kv4::mul2(y[i][k], inv2), kv4::widen(wt[i][k]));
-            if constexpr (!FULL) p[i][k] = kv4::mul2(kv4::mul2(p[i][k], inv2), kv4::widen(wt_other[i][k]));
+          for (int k = 0; k < 4; ++k) y[i][k] = kv4::mul2(kv4::mul2(y[i][k], inv2), wide[k]);
+          if constexpr (!FULL) {
+            widen8(wide, wt_other[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) p[i][k] = kv4::mul2(kv4::mul2(p[i][k], inv2), wide[k]);
           }
-      }
-      if constexpr (FULL) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) p[i][k] = y[1 - i][k];
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // added one by one: the compiler fuses a packed product and a packed sum
-          float a0, a1, b0, b1;
-          kv4::split2(kv4::mul2(y[i][k], cs[i][k]), a0, a1);
-          kv4::split2(kv4::mul2(p[i][k], sn[i][k]), b0, b1);
-          y[i][k] = kv4::make2(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
         }
+      }
+      // Products are added by an fma with a factor of one that the compiler does not know: it would fuse a packed
+      // product and a packed sum.
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (FULL) {
+          const f32x2 a = y[0][k], b = y[1][k];
+          y[0][k] = kv4::fma2(kv4::mul2(b, sn[0][k]), P.minus_one, kv4::mul2(a, cs[0][k]));
+          y[1][k] = kv4::fma2(kv4::mul2(a, sn[0][k]), P.one, kv4::mul2(b, cs[0][k]));
+        } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[i][k] = kv4::narrow(y[i][k]);
+          for (int i = 0; i < 2; ++i) {
+            const f32x2 o = kv4::fma2(kv4::mul2(p[i][k], sn[i][k]), P.one, kv4::mul2(y[i][k], cs[i][k]));
+            y[i][k] = turned[i] ? o : y[i][k];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) narrow8(x[i], y[i]);
       __nv_bfloat16* dst = nullptr;
       if (P.q_out == nullptr)
-        dst = src + static_cast<int64_t>(h) * HD;
+        dst = P.qkv + t * P.qkv_stride + static_cast<int64_t>((KIND == kQ ? 0 : P.hq) + h) * HD + 8 * l;
       else if (KIND == kQ)
         dst = P.q_out + (t * P.hq + h) * HD + 8 * l;
       else if (P.k_out != nullptr)
@@ -263,20 +298,25 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, int64_t t, int 
 
 template <int HD, bool KV4, bool FULL>
 __global__ void __launch_bounds__(kThreads, FULL ? 3 : 2) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
+  __shared__ int4 ring[kThreads / 32][kRing * 2 * 32];
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   if (item >= P.tokens * P.items_div.d) return;
   const int64_t t = P.items_div.div(static_cast<uint32_t>(item));
   const int begin = static_cast<int>(item - t * P.items_div.d) * P.steps_item;
-  const int end = begin + P.steps_item;
+  const int k0 = P.steps_q, v0 = k0 + P.steps_kv, end = min(begin + P.steps_item, v0 + P.steps_kv);
+  const Rows from{P, P.qkv + t * P.qkv_stride, ring[threadIdx.x >> 5] + (threadIdx.x & 31), end};
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i) from.load<HD>(begin + i);
   const int32_t pos = P.positions[t];
-  if (pos < 0 || pos >= P.max_pos) return;  // a token outside the table is left alone
-  uint8_t* cache_row = nullptr;
-  if (end > P.steps_q) cache_row = P.cache.row(P.slots[t]);
-
-  const int k0 = P.steps_q, v0 = k0 + P.steps_kv;
-  if (begin < k0) write_rows<HD, KV4, FULL, kQ>(P, t, begin, min(end, k0), pos, nullptr);
-  if (begin < v0 && end > k0) write_rows<HD, KV4, FULL, kK>(P, t, max(begin, k0) - k0, min(end, v0) - k0, pos, cache_row);
-  if (end > v0) write_rows<HD, KV4, FULL, kV>(P, t, max(begin, v0) - v0, min(end - v0, P.steps_kv), pos, cache_row);
+  if (pos >= 0 && pos < P.max_pos) {  // a token outside the table is left alone
+    uint8_t* cache_row = nullptr;
+    if (end > k0) cache_row = P.cache.row(P.slots[t]);
+    if (begin < k0) write_rows<HD, KV4, FULL, kQ>(P, from, t, 0, begin, min(end, k0), pos, nullptr);
+    if (begin < v0 && end > k0)
+      write_rows<HD, KV4, FULL, kK>(P, from, t, k0, max(begin, k0) - k0, min(end, v0) - k0, pos, cache_row);
+    if (end > v0) write_rows<HD, KV4, FULL, kV>(P, from, t, v0, max(begin, v0) - v0, end - v0, pos, cache_row);
+  }
+  kv4::copy_wait<0>();
 }
 
 // ---------------------------------------------------------------------------
@@ -370,6 +410,8 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   P.k_weight = static_cast<const __nv_bfloat16*>(k_weight);
   P.eps = eps;
   P.slots = slots;
+  P.one = 0x3f8000003f800000ull;
+  P.minus_one = 0xbf800000bf800000ull;
   P.q_out = static_cast<__nv_bfloat16*>(q_out);
   P.k_out = static_cast<__nv_bfloat16*>(k_out);
   if (hd != 64 && hd != 128 && hd != 256) return cudaErrorInvalidValue;

@@ -13,7 +13,8 @@ using kvbm::kv4::f32x2;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWriteThreads = 64;  // small blocks: their warps' places are taken up again sooner
+constexpr int kReadThreads = 128;
 
 // ---------------------------------------------------------------------------
 // q/k head norms + RoPE + paged cache write, one pass over a packed qkv.
@@ -296,10 +297,14 @@ __device__ __forceinline__ void write_rows(const WriteParams& P, const Rows& fro
   }
 }
 
+// Warps an SM holds: registers are for so many (80 and 128 a thread).
+constexpr int write_warps_sm(bool full) { return full ? 24 : 16; }
+
 template <int HD, bool KV4, bool FULL>
-__global__ void __launch_bounds__(kThreads, FULL ? 3 : 2) qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
-  __shared__ int4 ring[kThreads / 32][kRing * 2 * 32];
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kWriteThreads, write_warps_sm(FULL) * 32 / kWriteThreads)
+    qk_norm_rope_kv_write_kernel(const __grid_constant__ WriteParams P) {
+  __shared__ int4 ring[kWriteThreads / 32][kRing * 2 * 32];
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kWriteThreads / 32) + (threadIdx.x >> 5);
   if (item >= P.tokens * P.items_div.d) return;
   const int64_t t = P.items_div.div(static_cast<uint32_t>(item));
   const int begin = static_cast<int>(item - t * P.items_div.d) * P.steps_item;
@@ -336,10 +341,10 @@ struct GatherParams {
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads) kv4_gather_kernel(const __grid_constant__ GatherParams P) {
+__global__ void __launch_bounds__(kReadThreads) kv4_gather_kernel(const __grid_constant__ GatherParams P) {
   constexpr int L = HD / 16, R = 32 / L;
   const int lane = threadIdx.x & 31, l = lane % L, r = lane / L;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kReadThreads / 32) + (threadIdx.x >> 5);
   if (item >= P.tokens * P.items_div.d) return;
   const int64_t t = P.items_div.div(static_cast<uint32_t>(item));
   int group = static_cast<int>(item - t * P.items_div.d);
@@ -418,24 +423,26 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   const int rows_step = 512 / hd;
   P.steps_q = (hq + rows_step - 1) / rows_step;
   P.steps_kv = (hkv + rows_step - 1) / rows_step;
-  // a whole token a warp when there are warps enough to fill the GPU's 148 x 32 places; else its rows are spread
+  // A token's rows are spread over as many warps as find a place at the same time, and a warp has the whole token if
+  // tokens alone take all places (2,048 tokens of 32 + 16 heads of 128: whole tokens 13.6 us, two warps a token, of
+  // which the last ones wait for a place, 16.0; 512 tokens: six warps a token 5.1, four 5.6).
   const int steps = P.steps_q + 2 * P.steps_kv;
-  const int64_t items = std::min<int64_t>(steps, std::max<int64_t>(1, (2 * 148 * 32 + tokens - 1) / tokens));
+  const int64_t items = std::clamp<int64_t>(148 * write_warps_sm(rot == hd) / tokens, 1, steps);
   P.steps_item = static_cast<int>((steps + items - 1) / items);
   P.items_div = FastDiv(static_cast<uint32_t>((steps + P.steps_item - 1) / P.steps_item));
   const int64_t warps = tokens * P.items_div.d;
   if (warps > 0x7fffffff) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32));
+  const unsigned grid = static_cast<unsigned>((warps + kWriteThreads / 32 - 1) / (kWriteThreads / 32));
 #define KVBM_WRITE(HD)                                                                           \
   case HD:                                                                                       \
     if (bits == 4 && rot == HD)                                                                  \
-      qk_norm_rope_kv_write_kernel<HD, true, true><<<grid, kThreads, 0, stream>>>(P);            \
+      qk_norm_rope_kv_write_kernel<HD, true, true><<<grid, kWriteThreads, 0, stream>>>(P);            \
     else if (bits == 4)                                                                          \
-      qk_norm_rope_kv_write_kernel<HD, true, false><<<grid, kThreads, 0, stream>>>(P);           \
+      qk_norm_rope_kv_write_kernel<HD, true, false><<<grid, kWriteThreads, 0, stream>>>(P);           \
     else if (rot == HD)                                                                          \
-      qk_norm_rope_kv_write_kernel<HD, false, true><<<grid, kThreads, 0, stream>>>(P);           \
+      qk_norm_rope_kv_write_kernel<HD, false, true><<<grid, kWriteThreads, 0, stream>>>(P);           \
     else                                                                                         \
-      qk_norm_rope_kv_write_kernel<HD, false, false><<<grid, kThreads, 0, stream>>>(P);          \
+      qk_norm_rope_kv_write_kernel<HD, false, false><<<grid, kWriteThreads, 0, stream>>>(P);          \
     break;
   switch (hd) {
     KVBM_WRITE(64)
@@ -465,11 +472,11 @@ extern "C" int kvbm_kv4_gather(const void* kv, int64_t block_stride, int64_t out
   P.items_div = FastDiv(2 * static_cast<uint32_t>((steps + kReadFly - 1) / kReadFly));
   const int64_t warps = tokens * P.items_div.d;
   if (warps > 0x7fffffff) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>((warps + kThreads / 32 - 1) / (kThreads / 32));
+  const unsigned grid = static_cast<unsigned>((warps + kReadThreads / 32 - 1) / (kReadThreads / 32));
   switch (hd) {
-    case 64: kv4_gather_kernel<64><<<grid, kThreads, 0, stream>>>(P); break;
-    case 128: kv4_gather_kernel<128><<<grid, kThreads, 0, stream>>>(P); break;
-    case 256: kv4_gather_kernel<256><<<grid, kThreads, 0, stream>>>(P); break;
+    case 64: kv4_gather_kernel<64><<<grid, kReadThreads, 0, stream>>>(P); break;
+    case 128: kv4_gather_kernel<128><<<grid, kReadThreads, 0, stream>>>(P); break;
+    case 256: kv4_gather_kernel<256><<<grid, kReadThreads, 0, stream>>>(P); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();

@@ -36,10 +36,13 @@ constexpr int kReadThreads = 128;
 // (folding w into cos and sin, two of five products less an element, moved 4 codes
 // in a chunk of 8,192 tokens).
 // What bounds it is HBM for a prefill (the rows go in and out once), nearly
-// matched by the instructions of the norm, the rotation and the quantising: hence
-// the packed arithmetic, and the next step's loads in flight under each step. For
-// a decode step it is the latency of one token, so there a token's rows are
-// spread over warps. Rows are taken by kind (q, k, v), which keeps branches uniform.
+// matched by the instructions of the norm, the rotation and the quantising (250 a
+// step; at the HBM rate an SM issues 340): hence the packed arithmetic, and copies
+// of three steps in flight. For a decode step it is the latency of one token, so
+// there a token's rows are spread over warps. Rows are taken by kind (q, k, v),
+// which keeps branches uniform. Measured at 32 + 16 heads of 128, 4 bits: 8,192
+// tokens, 195 MB, 37.6 us = 5.2 TB/s (a plain copy of as many bytes: 32 us); 32
+// tokens 2.7 us.
 // ---------------------------------------------------------------------------
 struct WriteParams {
   __nv_bfloat16* qkv;
@@ -328,7 +331,8 @@ __global__ void __launch_bounds__(kWriteThreads, write_warps_sm(FULL) * 32 / kWr
 // Rows of the cache back to bf16: k_out[t][h] / v_out[t][h] = z + s c of slot
 // slots[t] (zeros for a slot outside the pool). HBM bounds it, 5 bits an element
 // in and 16 out: lanes hold rows as in the write, and a warp has kReadFly steps of
-// 512 / HD rows in flight.
+// 512 / HD rows in flight. Measured at 8 heads of 128: 16,384 tokens, 88 MB, 14.7
+// us = 6.0 TB/s; 77 tokens 2.2 us.
 // ---------------------------------------------------------------------------
 constexpr int kReadFly = 2;
 struct GatherParams {

@@ -23,9 +23,9 @@
 // (a - b / 16) of two q needs more bits than fp16 has: with up to 4 query heads on
 // a KV head (PAIR) it goes in two parts, in two of the 8 columns of a product, and
 // 2^-22 of it is lost at most; with 5 to 8 there are no columns to spare, and c1 is
-// taken alone at one shift more a word. Each group of 32 is two m16n8k16 products, whose fp32 sums take the group's scale; the zeros' part,
-// sum over g of z_g (sum of q_g), is one bf16 product more with the sums of q in
-// three bf16 parts.
+// taken alone at one shift more a word. Each group of 32 is two m16n8k16 products,
+// whose fp32 sums take the group's scale; the zeros' part, sum over g of z_g (sum
+// of q_g), is one bf16 product more with the sums of q in three bf16 parts.
 //
 // P V. Codes of two tokens are paired by one byte permute. The V scale goes into
 // the weight: p' = fp16(p s f), off by at most 2^-11 of it, with f a power of two
@@ -57,6 +57,13 @@
 // in a head-first pool the 16 rows are one run, and in a token-first one two warps
 // share the rows of two neighbouring heads (SHARED), one of them issuing, with a
 // barrier of the two where a tile's stage is given back.
+//
+// Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
+// 8,448 tokens 65.5 us = 5.3 TB/s, one of 131,072 37.3 us = 4.5 TB/s, one of 300
+// 7.7 us; each further byte costs what it costs in a copy (1.02 of it token-first,
+// 0.99 head-first), the rest is the start, the last round and the merge, about 12
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.4 us = 3.2 TB/s,
+// where 500 instructions a tile are the bound (1.35 of a copy a further byte).
 #pragma once
 
 #include "common.cuh"
@@ -446,7 +453,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         if (two != 0u && leads && !given_up && (lane >> 1) == (tile & 15)) {
           uint64_t* bar = &full[owner][tile & 1];
           mbar_arrive_expect_tx(bar, id >= 0 ? kStage : 0);
-          if (id >= 0) copy_unit(st + (lane & 1) * kStage, &map, P.flat ? at * (G::kRow / 8) : 0, SHARED ? kvh >> 1 : kvh, P.flat ? 0 : at, id, bar);
+          if (id >= 0)
+            copy_unit(st + (lane & 1) * kStage, &map, P.flat ? at * (G::kRow / 8) : 0, SHARED ? kvh >> 1 : kvh,
+                      P.flat ? 0 : at, id, bar);
         }
         return two;
       } else {  // every row looks its own page up
@@ -903,9 +912,10 @@ inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, 
   p.chunks = (hq / hkv + kHeads - 1) / kHeads;
   p.y_total = hkv * p.chunks;
   // Where requests are short and few, one KV head a CTA: its 8 streams of tokens take a request's 1,024 tokens in 4
-  // rounds, and nothing is cut (600 tokens of one request, 8 KV heads: 8.8 us in place of 10.5). Else as many as it has warps, an even
-  // number so that pairs can share copies, unless requests are so few that each would be cut into more than 80 parts
-  // (131,072 tokens of one request, 8 KV heads: 296 parts of 8 heads 40 us, 74 of two 37 us, 37 of one 47 us).
+  // rounds, and nothing is cut (600 tokens of one request, 8 KV heads: 8.8 us in place of 10.5). Else as many as it
+  // has warps, an even number so that pairs can share copies, unless requests are so few that each would be cut into
+  // more than 80 parts (131,072 tokens of one request, 8 KV heads: 296 parts of 8 heads 40 us, 74 of two 37 us, 37 of
+  // one 47 us).
   const int most = (hd == 256 ? 8 : 16) / kMaxWarps;  // registers allow 16 warps an SM (8 with 256 elements a head)
   const bool short_few = kStart + (max_tokens + 8 * kTile - 1) / (8 * kTile) <= kWhole &&
                          static_cast<int64_t>(batch) * p.y_total <= 2 * most * sm_count;

@@ -566,13 +566,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     }
 
     // ---- running state: of query head tig (PAIR) or 2 tig + n; m in the scores' unit before factor
-    float m[NH], l[NH], z[NH][NG];
+    float m[NH], ref[NH], l[NH], z[NH][NG];  // ref = m factor, 0 before there is an m
     float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24; odd i: that of i - 1 and 16 times i's
     float vf = pow2(100);  // f; the first tile sets it
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       m[n] = -INFINITY;
-      l[n] = 0.f;
+      ref[n] = l[n] = 0.f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         z[n][g] = 0.f;
@@ -670,8 +670,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
               s[u][r][n] = fmaf(bf_lo(par[r][g]), PAIR ? c[2 * r] + c[2 * r + 1] : c[2 * r + n], s[u][r][n]);
         }
       }
-      // ---- softmax
+      // ---- softmax. A tile without a new maximum, as most are after the first few, needs no sums scaled.
       float alpha[NH];
+      bool higher = false;
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
         if (!whole) {
@@ -681,24 +682,36 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
             for (int r = 0; r < 2; ++r)
               if (!((live >> (16 * u + 8 * r + gid)) & 1u)) s[u][r][n] = -INFINITY;
         }
-        float top = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
+        alpha[n] = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
+        higher |= alpha[n] > m[n];
+      }
+      if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = fmaxf(m[n], top);
-        const float ref = top == -INFINITY ? 0.f : top * factor[n];
-        alpha[n] = ex2(fmaf(m[n], factor[n], -ref));
-        m[n] = top;
-        l[n] *= alpha[n];
+        for (int n = 0; n < NH; ++n) {
+          float top = alpha[n];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) z[n][g] *= alpha[n];
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          top = fmaxf(m[n], top);
+          ref[n] = top == -INFINITY ? 0.f : top * factor[n];
+          alpha[n] = ex2(fmaf(m[n], factor[n], -ref[n]));
+          m[n] = top;
+          l[n] *= alpha[n];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) z[n][g] *= alpha[n];
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NH; ++n) alpha[n] = 1.f;
+      }
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            s[u][r][n] = ex2(fmaf(s[u][r][n], factor[n], -ref));
+            s[u][r][n] = ex2(fmaf(s[u][r][n], factor[n], -ref[n]));
             l[n] += s[u][r][n];
           }
-      }
       // ---- weights times V scales, as operands: PAIR columns are (head, group parity)
       uint32_t par[2][2][NG], bp[2][NB][2];
 #pragma unroll

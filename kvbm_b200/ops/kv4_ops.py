@@ -210,7 +210,7 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
     _rows_out(out, "out", (B, hq, hd), dev)
     with _lib.on_device(dev, stream) as st:
         if out is None:
-            out = q.new_empty((B, hq, hd))
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if B == 0:
             return out
         need, sms = _decode_plan(B, hq, hkv, hd, max_blocks * kv.shape[2], ctas, dev.index)

@@ -196,7 +196,7 @@ _KERNELS_PER_CALL = {
     "kvbm_rope_kv_push": 1, "kvbm_rope_kv_write_qout": 1, "kvbm_rope_kv_push_heads": 1,
     "kvbm_silu_mul": 1, "kvbm_paged_decode_attn": 2, "kvbm_paged_decode_attn_fused": 1, "kvbm_paged_decode_attn_simt": 2,
     "kvbm_batch_tables": 1, "kvbm_slot_map": 1, "kvbm_qk_norm_rope_kv_write": 1, "kvbm_kv4_gather": 1,
-    "kvbm_paged_decode_attn_kv4": 2,
+    "kvbm_paged_decode_attn_kv4": 1,  # and the merge, where requests may be cut
     "kvbm_skinny_gemm": 1, "kvbm_kv_multicast": 1, "kvbm_signal_multicast": 1,
 }
 _launches = 0

@@ -84,7 +84,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: t
     ``k_weight`` (bf16 [hd]) scale the normalised head; without one that norm is left out. ``cos_sin`` is fp32
     [max_position, rot]: cos then sin of the rotate-half convention over the first ``rot`` (a multiple of 16)
     elements. ``kv`` is bf16 (hd wide) or uint8 (:func:`row_bytes` wide: 4 bits); the cache takes k and v as
-    rounded to bf16, at ``slots`` (int64 [T], distinct; one outside the pool is not written).
+    rounded to bf16, at ``slots`` (int64 [T], distinct; one outside the pool is not written). Norm and rotation
+    are fp32, every operation rounded by itself.
 
     Without ``q_out`` q and k are rotated in place in ``qkv``. With ``q_out`` (bf16 [T, hq, hd]) ``qkv`` stays as
     it is: the rotated q go there and k to the cache and, if given, to ``k_out`` (bf16 [T, hkv, hd]). A token
@@ -222,6 +223,8 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
         _lib.call("kvbm_paged_decode_attn_kv4", q.data_ptr(), row_stride, *cache, block_table.data_ptr() or None,
                   block_table.stride(0), max_blocks, seq_lens.data_ptr(), B, hq, hkv, hd, softmax_scale, ctas, sms,
                   scratch.data_ptr() if need > 0 else None, out.data_ptr(), st)
+        if need > 0:
+            _lib.count_launches(1)
     return out
 
 

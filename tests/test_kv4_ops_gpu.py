@@ -7,7 +7,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from kvbm_b200.ops import kv4_ops, table_ops
+from kvbm_b200.ops import _lib, kv4_ops, table_ops
 from kvbm_b200.physical.layout import KvBlockLayout, KvLayout, LayoutConfig
 
 BF = torch.bfloat16
@@ -637,3 +637,15 @@ def test_attention_scratch_of_requests_that_are_cut():
         _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, scratch=scratch), q, vals, 0.1)
     with pytest.raises(ValueError, match="are needed"):
         kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, scratch=scratch[4:])
+
+
+def test_launches_are_counted():
+    kv, table, _ = _filled(1, [40], 2, 64, 16)
+    q = torch.zeros(1, 4, 64, dtype=BF, device="cuda")
+    wide = torch.zeros(1, 400, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    for t, n in ((table, 1), (wide, 2)):
+        assert (kv4_ops.kv4_decode_scratch(1, 4, 2, 64, t.shape[1] * 16) > 0) == (n == 2)
+        before = _lib.launch_count()
+        kv4_ops.paged_decode_attn_kv4(q, kv, t, _i32([40]), 0.1)
+        assert _lib.launch_count() - before == n

@@ -80,11 +80,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return d;
 }
 __device__ __forceinline__ f32x2 widen(uint32_t bf16x2) { return make2(bf_lo(bf16x2), bf_hi(bf16x2)); }
-__device__ __forceinline__ uint32_t narrow(f32x2 x) {
-  float lo, hi;
-  split2(x, lo, hi);
-  return pack2(lo, hi);
-}
 // NaN if either is.
 __device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;

@@ -97,6 +97,11 @@ struct AttnParams {
   bool flat;  // a head's rows in a page are contiguous: the copies take them as one
 };
 
+// A kernel launched by launch_overlapped reads and writes nothing before wait_before, the end of the kernel before;
+// release_next lets the next one be put in place.
+__device__ __forceinline__ void wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 constexpr int kHeads = 8;       // query heads a warp takes at most
 constexpr int kMaxWarps = 8;
 enum Copies { kRows, kTma, kTmaShared };
@@ -262,8 +267,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const __gri
   __shared__ float red[kMergeWarps][HD + 2];
   const int b = blockIdx.y, h_begin = blockIdx.x * heads_cta, h_end = min(P.hq, h_begin + heads_cta);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  release_next();
+  wait_before();
   const int2 parts = __ldcg(&P.parts[b]);
   const int n = parts.y;
   if (n == 1) return;  // written by its one CTA
@@ -330,7 +335,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  asm volatile("griddepcontrol.launch_dependents;");  // the merge may be put in place; it waits for this grid's end
+  release_next();  // the merge
   __shared__ uint64_t full[kMaxWarps][2];  // a warp's two tiles
   if constexpr (TMA) {
     if (lane < 2) mbar_init(&full[warp][lane], 2);  // the two lanes that issue its units
@@ -339,7 +344,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   }
 
   // What is above overlaps the end of the kernel before; nothing that it may have written is read above.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_before();
   // ---- this CTA's range of rounds, and the request it begins in
   __shared__ int64_t warp_sum[kMaxWarps];
   __shared__ int64_t cut_at[2], cut_first;

@@ -13,7 +13,7 @@
 // barriers), because a CTA that waited for another's scan would wait longer than
 // the scan takes; then rows and tokens are spread over the grid, and a token
 // finds its request by bisection in the scanned sums. Measured: 256 requests with
-// 8,192 tokens and rows of 1,024 blocks 4.1 us, 4 with 64 tokens 2.5 us; slots of
+// 8,192 tokens and rows of 1,024 blocks 4.0 us, 4 with 64 tokens 2.6 us; slots of
 // 32 tokens from a table 1.4 us.
 #include "common.cuh"
 #include "kvbm_kernels.h"

@@ -41,8 +41,8 @@ constexpr int kReadThreads = 128;
 // of three steps in flight. For a decode step it is the latency of one token, so
 // there a token's rows are spread over warps. Rows are taken by kind (q, k, v),
 // which keeps branches uniform. Measured at 32 + 16 heads of 128, 4 bits: 8,192
-// tokens, 195 MB, 37.6 us = 5.2 TB/s (a plain copy of as many bytes: 32 us); 32
-// tokens 2.7 us.
+// tokens, 195 MB, 38.0 us = 5.1 TB/s (a plain copy of as many bytes: 32 us); 32
+// tokens 2.6 us.
 // ---------------------------------------------------------------------------
 struct WriteParams {
   __nv_bfloat16* qkv;
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(kWriteThreads, write_warps_sm(FULL) * 32 / kWr
 // Rows of the cache back to bf16: k_out[t][h] / v_out[t][h] = z + s c of slot
 // slots[t] (zeros for a slot outside the pool). HBM bounds it, 5 bits an element
 // in and 16 out: lanes hold rows as in the write, and a warp has kReadFly steps of
-// 512 / HD rows in flight. Measured at 8 heads of 128: 16,384 tokens, 88 MB, 14.7
-// us = 6.0 TB/s; 77 tokens 2.2 us.
+// 512 / HD rows in flight. Measured at 8 heads of 128: 16,384 tokens, 88 MB, 14.0
+// us = 6.3 TB/s; 77 tokens 1.7 us.
 // ---------------------------------------------------------------------------
 constexpr int kReadFly = 2;
 struct GatherParams {

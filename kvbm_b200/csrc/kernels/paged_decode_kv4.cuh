@@ -59,10 +59,10 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 64.4 us = 5.4 TB/s, one of 131,072 36.8 us = 4.6 TB/s, one of 300
+// 8,448 tokens 64.8 us = 5.4 TB/s, one of 131,072 36.9 us = 4.5 TB/s, one of 300
 // 7.7 us; each further byte costs what it costs in a copy (1.00 of it token-first,
 // 0.99 head-first), the rest is the start, the last round and the merge, about 11
-// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.2 us = 3.2 TB/s,
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.1 us = 3.2 TB/s,
 // where 500 instructions a tile are the bound (1.3 of a copy a further byte, as at
 // 128 with 5 to 8 heads on one). Pages that are not a multiple of 16 tokens, whose
 // rows are copied one by one, cost 1.5 to 2.1.

@@ -28,10 +28,19 @@
 // of q_g), is one bf16 product more with the sums of q in three bf16 parts.
 //
 // P V. Codes of two tokens are paired by one byte permute. The V scale goes into
-// the weight: p' = fp16(p s f), off by at most 2^-11 of it, with f a power of two
-// that put the largest s f at [2^8, 2^9) when it was set; when sums of p' come out
-// infinite f is set again, and the sums of products with it. Then
+// the weight: p' = fp16(p s f), f a power of two. When sums of p' come out infinite,
+// as they do in a first tile, f is set so that the largest p s lies at [2^10, 2^11)
+// (2^9 with the most operands), and the sums of products go along. Then
 // sum p v = sum p' c / f + sum p z.
+// p' is off by up to 2^-11 of itself, or by 2^-25 / f. So the largest weight that a
+// query head has given a group of V has to lie at 2 or more, where the latter is
+// 2^-26 of it: a tile in which the head's maximum m rises, or in which f falls, has
+// to bring each group such a weight. Where one does not (V whose scales differ by a
+// factor of 2^9 or so), share_in_fp32 does the warp's tiles of this request again,
+// element by element. (A factor for each head and group took 4 to 22 % more time in
+// registers or in shared memory, with all tiles.) 11 bits are enough for the others:
+// a second fp16 part would double the products with 5 to 8 heads, and an average of
+// weights so rounded is nearer than the bf16 of the result.
 // Products of 32 tokens are folded into fp32 accumulators, since the tensor
 // core's own accumulation truncates.
 //
@@ -59,10 +68,10 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 64.8 us = 5.4 TB/s, one of 131,072 36.9 us = 4.5 TB/s, one of 300
-// 7.7 us; each further byte costs what it costs in a copy (1.00 of it token-first,
+// 8,448 tokens 66.1 us = 5.2 TB/s, one of 131,072 38.0 us = 4.4 TB/s, one of 300
+// 8.0 us; each further byte costs what it costs in a copy (1.00 of it token-first,
 // 0.99 head-first), the rest is the start, the last round and the merge, about 11
-// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.1 us = 3.2 TB/s,
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 34.0 us = 3.1 TB/s,
 // where 500 instructions a tile are the bound (1.3 of a copy a further byte, as at
 // 128 with 5 to 8 heads on one). Pages that are not a multiple of 16 tokens, whose
 // rows are copied one by one, cost 1.5 to 2.1.
@@ -194,6 +203,12 @@ __device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 __device__ __forceinline__ int exponent(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 255u) - 127; }
 
+// The same value, for a branch that is seldom taken: what is computed from it there is not moved in front of the branch.
+__device__ __forceinline__ uint32_t seldom(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+
 __device__ __forceinline__ int tokens_of(const AttnParams& P, int b) {
   return static_cast<int>(min(static_cast<int64_t>(max(P.seq_lens[b], 0)),
                               min(static_cast<int64_t>(P.max_blocks) * P.cache.page, static_cast<int64_t>(0x7ffff000))));
@@ -320,6 +335,103 @@ struct Geometry {
   static constexpr int kRingBytes = 4 * 2 * kUnit * kRow;  // a warp: two tiles of two units, K and V
 };
 
+// The K row (the V row is outer_stride behind it) of token t of a request, or null for a page outside the pool.
+__device__ __forceinline__ const uint8_t* row_of(const AttnParams& P, const int32_t* table, int t, int kvh) {
+  const uint32_t col = P.cache.page_div.div(static_cast<uint32_t>(t));
+  const int32_t id = table[col];
+  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(P.cache.num_blocks)) return nullptr;
+  return P.cache.base + id * P.cache.block_stride +
+         P.cache.page_div.mod(static_cast<uint32_t>(t), col) * P.cache.token_stride + kvh * P.cache.head_stride;
+}
+// Whether a group that any head lacks a large weight for has elements that differ, in any of a warp's tokens (groups of
+// equal elements, as in padding, take no weights; with one such group in four 105 us in place of 75).
+template <int HD, bool PAIR>
+__device__ __forceinline__ bool any_scale(const AttnParams& P, int b, int kvh, int seq, int t_begin, int tiles,
+                                          int round_tokens, uint32_t lacking) {
+  constexpr int NG = HD / kGroup;
+  lacking = __reduce_or_sync(0xffffffffu, lacking);
+  const int32_t* table = P.table + b * P.table_stride;
+  bool found = false;
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int t = t_begin + tile * round_tokens + static_cast<int>(threadIdx.x & 31);
+    const uint8_t* k = t < seq ? row_of(P, table, t, kvh) : nullptr;
+    if (k == nullptr) continue;
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t mine = PAIR ? (g & 1 ? 0x40000000u : 0x4000u) >> (g / 2) : 0x40004000u >> g;
+      if (lacking & mine)
+        found |= (*reinterpret_cast<const uint32_t*>(k + P.cache.outer_stride + HD / 2 + 4 * g) & 0xffffu) != 0u;
+    }
+  }
+  return __any_sync(0xffffffffu, found);
+}
+// A warp's tiles of a request once more, from the pool and in fp32 alone: a token at a time, each element taken apart.
+// Lane (gid, tig) has elements 32 g + 4 gid + i of query heads NH tig + n, as in the loop that it replaces (32
+// requests of 8,448 tokens, all of them again: 1.0 ms in place of 0.07. With the next token's rows under way it took
+// 0.8, and the registers for that 2 to 8 % of the other's time).
+template <int HD, int NH>
+__device__ __forceinline__ void share_in_fp32(const AttnParams& P, int b, int kvh, int head0, int heads, int seq,
+                                              int t_begin, int tiles, int round_tokens, float (&m)[NH], float (&l)[NH],
+                                              float (&acc)[HD / kGroup][4][NH]) {
+  constexpr int NG = HD / kGroup;
+  const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  float q[NH][NG][4];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint2 w = make_uint2(0u, 0u);
+      if (NH * tig + n < heads)
+        w = *reinterpret_cast<const uint2*>(P.q + b * P.q_stride + (head0 + NH * tig + n) * static_cast<int64_t>(HD) +
+                                            g * kGroup + gid * 4);
+      q[n][g][0] = bf_lo(w.x), q[n][g][1] = bf_hi(w.x), q[n][g][2] = bf_lo(w.y), q[n][g][3] = bf_hi(w.y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[g][i][n] = 0.f;
+    }
+  }
+  const int32_t* table = P.table + b * P.table_stride;
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int t0 = t_begin + tile * round_tokens;
+    for (int t = t0; t < min(seq, t0 + kTile); ++t) {
+      const uint8_t* k = row_of(P, table, t, kvh);
+      if (k == nullptr) continue;
+      const uint8_t* v = k + P.cache.outer_stride;
+      float score[NH], x[NG][4];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) score[n] = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t kc = *reinterpret_cast<const uint16_t*>(k + 16 * g + 2 * gid);
+        const uint32_t kp = *reinterpret_cast<const uint32_t*>(k + HD / 2 + 4 * g);
+        const uint32_t vc = *reinterpret_cast<const uint16_t*>(v + 2 * (NG * gid + g));
+        const uint32_t vp = *reinterpret_cast<const uint32_t*>(v + HD / 2 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = fmaf(static_cast<float>((kc >> (4 * i)) & 15u), bf_lo(kp), bf_hi(kp));
+          x[g][i] = fmaf(static_cast<float>((vc >> (4 * i)) & 15u), bf_lo(vp), bf_hi(vp));
+#pragma unroll
+          for (int n = 0; n < NH; ++n) score[n] = fmaf(q[n][g][i], y, score[n]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) score[n] += __shfl_xor_sync(0xffffffffu, score[n], o);
+        score[n] *= P.qscale;
+        const float top = fmaxf(m[n], score[n]), ref = top == -INFINITY ? 0.f : top;
+        const float down = exp2f(m[n] - ref), p = exp2f(score[n] - ref);
+        m[n] = top;
+        l[n] = fmaf(l[n], down, p);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[g][i][n] = fmaf(p, x[g][i], acc[g][i][n] * down);
+      }
+    }
+  }
+}
+
 template <int HD, bool PAIR, Copies COPIES>
 __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     kv4_decode_kernel(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap map) {
@@ -332,6 +444,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
   constexpr int NW = NG / 2;             // words of V codes a lane takes from a row
   constexpr int NZ = (NG + 3) / 4;       // products for the zeros of K
   constexpr int NB = PAIR ? NG / 2 : NG; // operands of weights a unit
+  constexpr int kBest = NB < 8 ? 10 : 9; // exponent of a tile's largest weight when f is set: 4 NB such add up to less than 2^16
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
@@ -576,6 +689,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     float m[NH], ref[NH], l[NH], z[NH][NG];  // ref = m factor, 0 before there is an m
     float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24; odd i: that of i - 1 and 16 times i's
     float vf = pow2(100);  // f; the first tile sets it
+    uint32_t lacking = 0u;         // the lane's heads' groups that have not been given a large weight where they should
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       m[n] = -INFINITY;
@@ -692,15 +806,17 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         alpha[n] = fmaxf(fmaxf(s[0][0][n], s[0][1][n]), fmaxf(s[1][0][n], s[1][1][n]));
         higher |= alpha[n] > m[n];
       }
-      if (__any_sync(0xffffffffu, higher)) {
+      higher = __any_sync(0xffffffffu, higher);
+      if (higher) {
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
           float top = alpha[n];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const bool rises = top > m[n];
           top = fmaxf(m[n], top);
           ref[n] = top == -INFINITY ? 0.f : top * factor[n];
-          alpha[n] = ex2(fmaf(m[n], factor[n], -ref[n]));
+          alpha[n] = rises ? ex2(fmaf(m[n], factor[n], -ref[n])) : 1.f;
           m[n] = top;
           l[n] *= alpha[n];
 #pragma unroll
@@ -731,7 +847,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
             for (int g = 0; g < NG; ++g) z[n][g] = fmaf(s[u][r][n], bf_hi(par[u][r][g]), z[n][g]);
         }
-      for (bool set = false;; set = true) {
+      bool set = false;
+      while (true) {
         uint32_t sum = 0u;  // infinite (or a NaN) if a weight is, or all are near it
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -753,24 +870,30 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           }
         const bool over = (sum & 0x7c00u) == 0x7c00u || (sum & 0x7c000000u) == 0x7c000000u;
         if (set || !__any_sync(0xffffffffu, over)) break;
+        set = true;
         float top = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int g = 0; g < NG; ++g) top = fmaxf(top, bf_lo(par[u][r][g]));
+            for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float next_vf = fminf(vf, pow2(min(max(8 - exponent(top), -126), 100)));
-        const float down = next_vf / vf;
-        vf = next_vf;
+              for (int g = 0; g < NG; ++g) top = fmaxf(top, s[u][r][n] * bf_lo(seldom(par[u][r][g])));
+        const int old = exponent(vf), now = min(old, kBest - exponent(warp_max(top)));
+        vf = pow2(now);
 #pragma unroll
-        for (int n = 0; n < NH; ++n)
+        for (int n = 0; n < NH; ++n) alpha[n] *= pow2(max(now - old, -126));
+      }
+      if (higher || set) {  // has each group been given a weight of 2 or more, bit 14 of an fp16?
+        constexpr uint32_t kLow = 0x4000u / (1u << (NB - 1)) * ((1u << NB) - 1u);  // operand k: bits 14 - k, 30 - k
+        uint32_t have = (alpha[0] == 1.f ? kLow : 0u) | (alpha[NH - 1] == 1.f ? kLow << 16 : 0u);
 #pragma unroll
-          for (int g = 0; g < NG; ++g)
+        for (int k = 0; k < NB; ++k)
+          have |= ((bp[0][k][0] | bp[0][k][1] | bp[1][k][0] | bp[1][k][1]) & 0x40004000u) >> k;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[g][i][n] *= down;
+        for (int o = 4; o < 32; o <<= 1) have |= __shfl_xor_sync(0xffffffffu, have, o);
+        lacking |= (kLow | kLow << 16) & ~have;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -853,6 +976,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           acc[g][i][n] = fmaf(acc[g][i][n] * 16777216.f, 1.f / vf, z[n][g]);
         }
     }
+    if (__any_sync(0xffffffffu, lacking != 0u) && !given_up &&
+        any_scale<HD, PAIR>(P, b, kvh, seq, t_begin, mine, round_tokens, lacking))
+      share_in_fp32<HD, NH>(P, b, kvh, head0, heads, seq, t_begin, mine, round_tokens, m, l, acc);
     // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
     if (P.streams > 1) {
       constexpr int kVals = NH * (2 + 4 * NG);

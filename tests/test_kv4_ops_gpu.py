@@ -649,3 +649,100 @@ def test_launches_are_counted():
         before = _lib.launch_count()
         kv4_ops.paged_decode_attn_kv4(q, kv, t, _i32([40]), 0.1)
         assert _lib.launch_count() - before == n
+
+
+def _held(x, page=16):
+    """A pool with the rows of bf16 x [n, 2, heads, hd] as one request's, its table, the values in 64 bits and V's
+    scales [n, heads, hd]."""
+    n, _, heads, hd = x.shape
+    nb = -(-n // page)
+    rk, rv = kv4_ops.pack_rows(x[:, 0], False), kv4_ops.pack_rows(x[:, 1], True)
+    kv = _empty_pool(nb, page, heads, hd, fill=255)
+    for o, rows in ((0, rk), (1, rv)):
+        at = torch.arange(n, device="cuda")
+        kv[at // page, o, at % page] = rows
+    scales = rv[..., hd // 2: hd // 2 + hd // 8].contiguous().view(BF).double()[..., ::2].repeat_interleave(32, -1)
+    return kv, torch.arange(nb, dtype=torch.int32, device="cuda").view(1, nb), [_values(rk, rv)], scales
+
+
+def _spread_values(kind, n, heads, hd):
+    """V whose scales differ, and K that make some tokens' scores the lowest by far."""
+    x = torch.randn(n, 2, heads, hd, device="cuda", generator=_gen(hd + n))
+    if kind == "one group":              # a group of channels far above its neighbours
+        x[:, 1, :, :32] *= 1e10
+    elif kind == "one group 60 times":
+        x[:, 1, :, :32] *= 60
+    elif kind == "one group far below":
+        x[:, 1, :, 32:] *= 1e-12
+    elif kind == "later tokens":         # what was summed before has to be brought down
+        x[n // 2:, 1] *= 2.0 ** 15
+    elif kind == "later tokens of a group":
+        x[n // 3:, 1, :, :32] *= 1e9
+    elif kind == "first tokens that hardly count":  # they alone set how the weights are held, at first
+        x[:40, 1] *= 1e20
+        x[:40, 0, :, 0] = -800.0
+        x[40:, 0, :, 0] = 20.0
+    elif kind == "a light token among others":
+        x[5, 1] *= 1e15
+        x[5, 0, :, 0] = -800.0
+    elif kind == "a group of equal elements":
+        x[:, 1, :, 32:64] = 0.5
+    elif kind == "equal elements at first":
+        x[:500, 1, :, :32] = 0.25
+        x[500:, 1, :, :32] *= 1e-7
+    elif kind == "tiny":
+        x[:, 1] *= 1e-33
+    return x.to(BF)
+
+
+@pytest.mark.parametrize("group,hd", [(4, 128), (7, 64), (2, 256), (8, 128), (6, 256), (1, 64)])
+@pytest.mark.parametrize("kind", ["one group", "one group 60 times", "one group far below", "later tokens",
+                                  "later tokens of a group", "first tokens that hardly count",
+                                  "a light token among others", "a group of equal elements",
+                                  "equal elements at first", "tiny"])
+def test_attention_values_of_very_different_size(kind, group, hd):
+    """Each group of V against its own size. Beside what `_values` allows, a weight may be off by 2^-26 of the largest
+    that the head gives the group, times a code of up to 15."""
+    n, heads = 700, 2
+    kv, table, vals, scales = _held(_spread_values(kind, n, heads, hd))
+    q = torch.randn(1, heads * group, hd, device="cuda", generator=_gen(group)).to(BF)
+    q[..., 0] = 1.0
+    scale = 1 / math.sqrt(hd)
+    want, size = _attn64(q, vals, scale)
+    k = vals[0][0].repeat_interleave(group, 1)
+    p = torch.softmax(torch.einsum("hd,nhd->hn", q[0].double(), k) * scale, -1)
+    largest = (p.t().unsqueeze(-1) * scales.repeat_interleave(group, 1)).amax(0)
+    size = size + 15 * n * 2.0 ** -26 * largest
+    for ctas in (1, 4):
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), scale, ctas=ctas)
+        # rounded to bf16 once
+        assert ((got.double() - want).abs() <= HALF_STEP * (want.abs() + size) + size + 2.0 ** -133).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_one_token_far_above_many_whose_values_vary(hd):
+    """As above where the many tokens' values fill their groups, so that their weights are held in 16 bits."""
+    n = 4096
+    x = torch.randn(n, 2, 1, hd, device="cuda", generator=_gen(hd))
+    x[:, 0] = 0.0
+    x[0, 0, 0, 0] = 8.0
+    kv, table, vals, _ = _held(x.to(BF))
+    q = torch.zeros(1, 1, hd, device="cuda", dtype=BF)
+    q[0, 0, 0] = 1.0
+    for ctas in (1, 8):
+        _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, ctas=ctas), q, vals, 1.0)
+
+
+def test_attention_poisoned_value_shows_only_where_it_is():
+    """A V row with a NaN in one group: this group of the heads that read it, and no other result."""
+    lens, hkv, hd = [40, 40], 2, 128
+    kv, table, vals = _filled(2, lens, hkv, hd, 16, seed=13)
+    x = torch.randn(1, hd, device="cuda", generator=_gen(1)).to(BF)
+    x[0, 70] = math.nan
+    kv[int(table[0, 1]), 1, 3, 1] = kv4_ops.pack_rows(x, True)[0]
+    q = torch.randn(2, 4, hd, device="cuda", generator=_gen(4)).to(BF)
+    got = kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32(lens), 0.1, ctas=3)
+    assert got[0, 2:, 64:96].isnan().all()
+    assert got[0, 2:, :64].isfinite().all() and got[0, 2:, 96:].isfinite().all()
+    assert got[0, :2].isfinite().all()
+    _check_attn(got[1:], q[1:], vals[1:], 0.1)

@@ -198,9 +198,9 @@ extern "C" int kvbm_batch_tables(const int32_t* query_lens, const int32_t* conte
   P.page = page;
   P.page_div = FastDiv(static_cast<uint32_t>(page));
   const size_t smem = 2 * sizeof(int64_t) * (static_cast<size_t>(batch) + 1);
-  if (smem > 48 * 1024) {
+  if (smem > 48 * 1024) {  // for the largest batch: another thread's launch may stand between this call and the launch
     const cudaError_t e = cudaFuncSetAttribute(batch_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+                                               static_cast<int>(2 * sizeof(int64_t) * (kMaxBatch + 1)));
     if (e != cudaSuccess) return e;
   }
   // a row or 256 tokens a CTA, up to four CTAs on each of 148 SMs

@@ -1134,10 +1134,12 @@ cudaError_t launch_decode_kernel(const AttnParams& P, const CUtensorMap& map, co
   auto kernel = kv4_decode_kernel<HD, PAIR, COPIES>;
   const int warps = plan.y_cta * plan.streams;
   constexpr int kVals = (PAIR ? 1 : 2) * (2 + 4 * (HD / kGroup));  // merging streams, in the ring's place
-  const int smem = warps * std::max(Geometry<HD>::kRingBytes, kVals * 128);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr int kWarpBytes = std::max(Geometry<HD>::kRingBytes, kVals * 128);
+  // what any launch may take: another thread's launch of this kernel may stand between this call and the next
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxWarps * kWarpBytes);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kernel, dim3(plan.ctas, plan.y_ctas), warps * 32, smem, stream, P, map);
+  return launch_overlapped(kernel, dim3(plan.ctas, plan.y_ctas), warps * 32, warps * kWarpBytes, stream, P, map);
 }
 
 template <int HD>

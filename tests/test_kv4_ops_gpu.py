@@ -1,6 +1,7 @@
 """GPU numerics of the 4-bit cache's operators against plain forms in 64 bits."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -746,3 +747,52 @@ def test_attention_poisoned_value_shows_only_where_it_is():
     assert got[0, 2:, :64].isfinite().all() and got[0, 2:, 96:].isfinite().all()
     assert got[0, :2].isfinite().all()
     _check_attn(got[1:], q[1:], vals[1:], 0.1)
+
+
+def _in_threads(calls, rounds):
+    """Each of `calls` over and over in a thread of its own; what they raised."""
+    errors = []
+
+    def work(call):
+        try:
+            for _ in range(rounds):
+                call()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return errors
+
+
+def test_attention_calls_of_several_threads():
+    """Launches of one kernel that take different amounts of shared memory (a request with a short table 8 warps a CTA,
+    four with long ones 6) do not get in each other's way."""
+    kv, table, vals = _filled(1, [40], 6, 128, 16, "hnd")
+    one = torch.randn(1, 6, 128, device="cuda", generator=_gen(1)).to(BF)
+    wide = torch.zeros(4, 400, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    outs = []
+
+    def call(t):
+        q, seq = one.expand(t.shape[0], 6, 128).contiguous(), _i32([40] * t.shape[0])
+        out, scratch = torch.empty_like(q), torch.empty(1 << 20, device="cuda")
+        outs.append(out)
+        return lambda: kv4_ops.paged_decode_attn_kv4(q, kv, t, seq, 0.1, out=out, scratch=scratch)
+
+    assert not _in_threads([call(table), call(wide), call(table), call(wide)], 500)
+    for out in outs:
+        for row in out:
+            _check_attn(row[None], one, vals, 0.1)
+
+
+def test_table_calls_of_several_threads():
+    def call(B):
+        q, c, ids = torch.ones(B, dtype=torch.int32, device="cuda"), _i32([0] * B), torch.arange(B, dtype=torch.int32, device="cuda")
+        return lambda: table_ops.batch_tables(q, c, ids, page=16, max_blocks=1)
+
+    assert not _in_threads([call(8192), call(3500), call(8192), call(3500)], 500)

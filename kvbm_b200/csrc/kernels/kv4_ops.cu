@@ -406,7 +406,7 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   P.cache = Cache{static_cast<uint8_t*>(kv), block_stride, outer_stride, token_stride, head_stride, page, num_blocks, hkv,
                   FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (tokens < 0 || hq < 0 || !cache_ok(P.cache) || !qkv || !positions || !cos_sin || !slots || !aligned16(qkv) ||
-      qkv_stride % 8 != 0 || !aligned16(cos_sin) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(q_weight) ||
+      (tokens > 1 && qkv_stride % 8 != 0) || !aligned16(cos_sin) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(q_weight) ||
       !aligned16(k_weight) || rot <= 0 || rot > hd || rot % 16 != 0 || max_pos < 0 || (bits != 4 && bits != 16) ||
       (k_out && !q_out))
     return cudaErrorInvalidValue;
@@ -512,7 +512,7 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
   P.cache = Cache{static_cast<uint8_t*>(const_cast<void*>(kv)), block_stride, outer_stride, token_stride, head_stride,
                   page, num_blocks, hkv, FastDiv(static_cast<uint32_t>(page > 0 ? page : 1))};
   if (batch < 0 || batch > 65535 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || !cache_ok(P.cache) || !q || !aligned16(q) ||
-      q_stride % 8 != 0 || !out || !aligned16(out) || !seq_lens || max_blocks < 0 || (max_blocks > 0 && !block_table) ||
+      (batch > 1 && q_stride % 8 != 0) || !out || !aligned16(out) || !seq_lens || max_blocks < 0 || (max_blocks > 0 && !block_table) ||
       ctas < 0 || sm_count <= 0 || !aligned16(scratch))
     return cudaErrorInvalidValue;
   const kv4::Plan plan =

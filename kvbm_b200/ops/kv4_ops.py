@@ -42,6 +42,8 @@ def _cache_args(kv: torch.Tensor, device, bits: int = 4) -> tuple:
         raise ValueError(f"a {bits}-bit cache is {torch.uint8 if bits == 4 else torch.bfloat16}, not {kv.dtype}")
     nb, _, page, heads, row = kv.shape
     block, outer, token, head, unit = kv.stride()
+    # a dimension of one may come with any stride
+    block, token, head = block if nb > 1 else 0, token if page > 1 else 0, head if heads > 1 else 0
     ptr = kv.data_ptr()
     if bits == 16:
         block, outer, token, head = 2 * block, 2 * outer, 2 * token, 2 * head

@@ -796,3 +796,35 @@ def test_table_calls_of_several_threads():
         return lambda: table_ops.batch_tables(q, c, ids, page=16, max_blocks=1)
 
     assert not _in_threads([call(8192), call(3500), call(8192), call(3500)], 500)
+
+
+def test_strides_of_dimensions_of_one_do_not_matter():
+    """One token, one request, one block, page or head may lie at any pitch: it is not used."""
+    hd, hkv, page = 128, 2, 16
+    kv, table, vals = _filled(1, [30], hkv, hd, page)
+    q = torch.randn(1, 8, hd, device="cuda", generator=_gen(3)).to(BF)
+    odd = torch.zeros(1, 8 * hd + 3, dtype=BF, device="cuda")
+    odd[:, : 8 * hd] = q.flatten(1)
+    view = odd.as_strided((1, 8, hd), (8 * hd + 3, hd, 1))
+    assert view.stride(0) % 8
+    _check_attn(kv4_ops.paged_decode_attn_kv4(view, kv, table, _i32([30]), 0.1), q, vals, 0.1)
+    x = torch.randn(1, 8, hd, device="cuda", generator=_gen(4)).to(BF)
+    odd[:, : 8 * hd] = x.flatten(1)
+    where, cs, slot = _i32([0]), _cos_sin(1, hd), torch.tensor([5], device="cuda")
+    a, b = _empty_pool(1, page, hkv, hd), _empty_pool(1, page, hkv, hd)
+    qa, qb = torch.empty(2, 1, 4, hd, dtype=BF, device="cuda")
+    kv4_ops.qk_norm_rope_kv_write(x, where, cs, 4, hkv, a, slot, q_out=qa)
+    kv4_ops.qk_norm_rope_kv_write(view, where, cs, 4, hkv, b, slot, q_out=qb)
+    assert torch.equal(a, b) and torch.equal(qa, qb)
+    # one block of one head, as a slice of bytes at odd pitches
+    flat = torch.zeros(3 * page * 80 + 40, dtype=torch.uint8, device="cuda")
+    one = flat.as_strided((1, 2, page, 1, 80), (24, page * 80, 80, 7, 1))
+    rows = torch.empty(1, 2, page, 1, 80, dtype=torch.uint8, device="cuda")
+    rows.copy_(kv[int(table[0, 0]), :, :, :1][None])
+    one.copy_(rows)
+    at = torch.arange(page, device="cuda")
+    for got, want in zip(kv4_ops.kv4_gather(one, at), kv4_ops.kv4_gather(rows, at)):
+        assert torch.equal(got, want)
+    q1 = q[:, :4].contiguous()
+    _check_attn(kv4_ops.paged_decode_attn_kv4(q1, one, _i32([[0]]), _i32([page]), 0.1), q1,
+                [tuple(x[:page, :1] for x in vals[0])], 0.1)

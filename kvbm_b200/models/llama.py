@@ -210,7 +210,9 @@ class LlamaModel:
         self.cos_sin = torch.cat([f.cos(), f.sin()], dim=-1).float().to(self.device)
         self.scale = 1.0 / math.sqrt(c.head_dim)
         self._decode_scratch: torch.Tensor | None = None
-        self._outgrown: list = []
+        self._scratch_captured = False          # a captured step has been given the present one
+        self._scratch_stream: torch.cuda.Stream | None = None
+        self._outgrown: list[torch.Tensor] = []  # earlier ones that captured steps go on using
         self._decode_counters: torch.Tensor | None = None
         self.decode_gemm = "cublas"  # "tc": decode projections on the tcgen05 skinny GEMM
         self._gemm_ws: llama_ops.GemmWorkspace | None = None
@@ -361,10 +363,25 @@ class LlamaModel:
     def decode_scratch(self, batch: int, splits: int) -> torch.Tensor:
         return self._scratch(batch * self.cfg.heads * splits * (self.cfg.head_dim + 2))
 
+    def _capturing(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
     def _scratch(self, need: int) -> torch.Tensor:
-        if self._decode_scratch is None or self._decode_scratch.numel() < need:
-            self._outgrown.append(self._decode_scratch)  # a captured step goes on using it
-            self._decode_scratch = torch.empty(need, dtype=torch.float32, device=self.device)
+        """``need`` floats that the decode steps share. It grows by half at least, so that a batch that grows by one
+        request at a time does not make one for each; an outgrown one is kept only if a captured step was given it."""
+        have = 0 if self._decode_scratch is None else self._decode_scratch.numel()
+        capturing = self._capturing()
+        if self._decode_scratch is None or have < need:
+            if self._scratch_captured:
+                self._outgrown.append(self._decode_scratch)
+            self._decode_scratch = torch.empty(max(need, have + have // 2), dtype=torch.float32, device=self.device)
+            self._scratch_captured = False
+            self._scratch_stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+        elif self._scratch_stream is not None and not capturing:
+            stream = torch.cuda.current_stream(self.device)
+            if stream != self._scratch_stream:  # let go while a step on this stream still runs, it is not handed on
+                self._decode_scratch.record_stream(stream)
+        self._scratch_captured |= capturing
         return self._decode_scratch
 
     def dlinear(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
@@ -390,6 +407,7 @@ class LlamaModel:
         (position of each input token), block_table [B, max_blocks] int32,
         seq_lens [B] int32 (= positions + 1). Returns next tokens [B] int64.
         All shapes static, so the step can be captured in a CUDA graph.
+        Steps of one model share its workspaces: they run one after another, captured or not.
         ``splits`` is for 16-bit pools; over 4 bits the work is cut evenly on the device."""
         c = self.cfg
         B = tokens.numel()

@@ -6,6 +6,9 @@
 #include "paged_decode_kv4.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
 
 using namespace kvbm;
 using kvbm::kv4::Cache;
@@ -393,6 +396,37 @@ bool cache_ok(const Cache& c) {
          c.token_stride % 16 == 0 && c.head_stride % 16 == 0 && c.page > 0 && c.num_blocks >= 0 && c.heads > 0;
 }
 
+// One status word a device in mapped host memory: the host reads it without waiting for the device.
+constexpr int kMaxDevices = 64;
+std::mutex g_status_lock;
+std::atomic<int*> g_status_host{nullptr};
+std::atomic<uint64_t> g_wait_ns{kv4::kWaitNs};
+
+int* status_word() {
+  int* host = g_status_host;
+  if (host == nullptr) {
+    std::lock_guard<std::mutex> lock(g_status_lock);
+    host = g_status_host;
+    if (host == nullptr) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be one that is captured
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void* p = nullptr;
+      const cudaError_t e = cudaHostAlloc(&p, sizeof(int) * kMaxDevices, cudaHostAllocMapped | cudaHostAllocPortable);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (e != cudaSuccess) return nullptr;
+      host = static_cast<int*>(p);
+      std::memset(host, 0, sizeof(int) * kMaxDevices);
+      g_status_host = host;
+    }
+  }
+  int dev = 0;
+  void* d = nullptr;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices ||
+      cudaHostGetDevicePointer(&d, host + dev, 0) != cudaSuccess)
+    return nullptr;
+  return static_cast<int*>(d);
+}
+
 }  // namespace
 
 extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t tokens, int hq, int hkv, int hd,
@@ -539,16 +573,18 @@ extern "C" int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const
     P.parts = reinterpret_cast<int2*>(scratch + rows * (hd + 2));
   }
   P.out = static_cast<__nv_bfloat16*>(out);
+  P.status = status_word();
+  P.wait_ns = g_wait_ns;
+  if (P.status == nullptr) return cudaErrorMemoryAllocation;
   return kv4::launch_decode(P, hd, plan, stream);
 }
 
-// 0, or the status a launch recorded (3 = a wait for a copy gave up); synchronizes.
-extern "C" int kvbm_kv4_status(int reset) {
-  int v = -1;
-  if (cudaMemcpyFromSymbol(&v, kv4::g_kv4_status, sizeof(int)) != cudaSuccess) return -1;
-  if (reset) {
-    const int zero = 0;
-    cudaMemcpyToSymbol(kv4::g_kv4_status, &zero, sizeof(int));
-  }
+extern "C" int kvbm_kv4_status(int device, int reset) {
+  if (device < 0 || device >= kMaxDevices || g_status_host == nullptr) return 0;
+  volatile int* word = g_status_host + device;
+  const int v = *word;
+  if (reset) *word = 0;
   return v;
 }
+
+extern "C" void kvbm_kv4_set_wait_limit_ns(int64_t ns) { g_wait_ns = ns < 0 ? kv4::kWaitNs : static_cast<uint64_t>(ns); }

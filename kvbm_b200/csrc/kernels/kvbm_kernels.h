@@ -235,8 +235,11 @@ int kvbm_paged_decode_attn_kv4(const void* q, int64_t q_stride, const void* kv, 
                                int num_blocks, const int32_t* block_table, int64_t table_stride, int max_blocks,
                                const int32_t* seq_lens, int batch, int hq, int hkv, int hd, float softmax_scale,
                                int ctas, int sm_count, float* scratch, void* out, cudaStream_t stream);
-// 0, or 3 when a launch of the attention gave a copy up (its result is NaN); synchronizes.
-int kvbm_kv4_status(int reset);
+// 0, or 3 when a launch of the attention on `device` gave a copy up (its result is NaN): a host read of mapped memory,
+// no synchronization.
+int kvbm_kv4_status(int device, int reset);
+// After how long a launch from here on gives a copy up: 0 at once, negative the default of a second.
+void kvbm_kv4_set_wait_limit_ns(int64_t ns);
 
 #ifdef __cplusplus
 }

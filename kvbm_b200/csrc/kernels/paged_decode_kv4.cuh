@@ -103,6 +103,8 @@ struct AttnParams {
   float* part_ml;   // [cta][2][hq][2]
   int2* parts;      // [batch], null if no request can be cut: a request's first slot of partial results (2 cta, + 1: not its CTA's first), and how many
   __nv_bfloat16* out;
+  int* status;       // where a launch that gives a copy up says so
+  uint64_t wait_ns;  // after which a warp gives a copy up; 0: at once
   bool flat;  // a head's rows in a page are contiguous: the copies take them as one
 };
 
@@ -118,9 +120,7 @@ constexpr int kUnit = 16;       // tokens a stage of the ring holds
 constexpr int kTile = 32;       // tokens a warp takes between two updates of its accumulators
 constexpr int kMinRounds = 2;   // a CTA takes at least so many tiles a warp: below, merging costs more than it saves
 constexpr int kWhole = 6;       // requests of up to so many rounds (kStart among them) are not cut
-constexpr uint64_t kWaitNs = 1000000000ull;  // after which a warp gives a copy up
-
-__device__ int g_kv4_status = 0;
+constexpr uint64_t kWaitNs = 1000000000ull;  // limit of a wait for a copy
 
 // ---- instructions ----------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) {
@@ -714,12 +714,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         if (!given_up) {
           uint64_t* bar = &full[owner][tile & 1];
           const uint32_t phase = (phases >> (tile & 1)) & 1u;
-          bool ok = mbar_try_wait(bar, phase);
+          bool ok = P.wait_ns != 0 && mbar_try_wait(bar, phase);
           if (!__all_sync(0xffffffffu, ok)) {
-            ok = mbar_wait_bounded(bar, phase, kWaitNs);
+            ok = P.wait_ns != 0 && mbar_wait_bounded(bar, phase, P.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) {  // the launch is given up when both copies in flight have had their time
               given_up = true;
-              report_status(&g_kv4_status, kStatusPipelineTimeout);
+              report_status(P.status, kStatusPipelineTimeout);
               mbar_wait_bounded(bar, phase, kWaitNs);
               if (next != 0u) mbar_wait_bounded(&full[owner][~tile & 1], (phases >> (~tile & 1)) & 1u, kWaitNs);
             }

@@ -147,7 +147,8 @@ _SIGS = {
         [_VP, _I64, _VP, _I64, _I64, _I64, _I64, _INT, _INT, _VP, _I64, _INT, _VP, _INT, _INT, _INT, _INT, _F32, _INT,
          _INT, _VP, _VP, _VP],
     ),
-    "kvbm_kv4_status": (_INT, [_INT]),
+    "kvbm_kv4_status": (_INT, [_INT, _INT]),
+    "kvbm_kv4_set_wait_limit_ns": (None, [_I64]),
     "kvbm_skinny_gemm": (_INT, [_VP, _INT, _VP, _INT, _VP, _INT, _INT, _INT, _INT, _INT, _VP, _VP, _VP]),
     "kvbm_skinny_gemm_ctas": (_INT, []),
     "kvbm_skinny_gemm_set_pdl": (_INT, [_INT]),

@@ -184,7 +184,8 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
     page whose id is outside the pool holds no tokens. The work is cut evenly over ``ctas`` CTAs (0: as many as
     the GPU holds at a time), whatever the lengths; results of requests that several CTAs share go through
     ``scratch`` (fp32, :func:`kv4_decode_scratch` entries; made here if not given, nothing in it outlives the
-    call). Launches that may overlap need a scratch each.
+    call). Launches that may overlap need a scratch each. A launch whose copies do not arrive gives up: its results
+    are NaN, and :func:`check_kv4_status` raises.
     """
     if q.dim() != 3 or q.dtype != torch.bfloat16:
         raise ValueError("q must be bf16 [B, Hq, hd]")
@@ -230,10 +231,31 @@ def paged_decode_attn_kv4(q: torch.Tensor, kv: torch.Tensor, block_table: torch.
     return out
 
 
-def kv4_status(reset: bool = True) -> int:
-    """0, or the error a :func:`paged_decode_attn_kv4` launch recorded (3: a wait for a copy timed out; its results
-    are NaN) on the current device. Synchronizes."""
-    return int(_lib.load().kvbm_kv4_status(1 if reset else 0))
+def _index(device) -> int:
+    dev = torch.device(device) if device is not None else None
+    return dev.index if dev is not None and dev.index is not None else torch.cuda.current_device()
+
+
+def kv4_status(reset: bool = True, device=None) -> int:
+    """0, or the error a :func:`paged_decode_attn_kv4` launch recorded on ``device`` (None: the current one) since the
+    last reset; 3: a wait for a copy timed out, and the launch's results are NaN. Synchronizes the device."""
+    dev = _index(device)
+    torch.cuda.synchronize(dev)
+    return int(_lib.load().kvbm_kv4_status(dev, 1 if reset else 0))
+
+
+def check_kv4_status(device=None) -> None:
+    """Raise (and clear the status) if a :func:`paged_decode_attn_kv4` launch on ``device`` recorded an error. A host
+    read of mapped memory without synchronization: it sees the launches that the host has waited for."""
+    st = int(_lib.load().kvbm_kv4_status(_index(device), 1))
+    if st:
+        raise _lib.KvbmCudaError(f"decode attention over a 4-bit cache failed on the device: status {st} "
+                                 "(a wait for a copy timed out; the results of that launch are NaN)")
+
+
+def set_kv4_wait_limit_ns(ns: int | None) -> None:
+    """After how long a launch from here on gives a copy up: 0 at once, None the default of one second."""
+    _lib.load().kvbm_kv4_set_wait_limit_ns(-1 if ns is None else int(ns))
 
 
 # ------------------------------------------------------------- rows on the host

@@ -44,7 +44,7 @@ from ..connector.worker import ConnectorWorker
 from ..logical.manager import BlockManager, MutableBlock, Tier
 from ..logical.sequence import sequence_hashes
 from ..models.llama import LlamaModel
-from ..ops import llama_ops, table_ops
+from ..ops import kv4_ops, llama_ops, table_ops
 from ..physical.layout import KvLayout
 
 
@@ -256,6 +256,7 @@ class LLMEngine:
             bits = {} if cfg.kv_bits == 16 else {"kv_bits": cfg.kv_bits}
             pool = model.allocate_pool(cfg.num_gpu_blocks, cfg.block_size, **bits)
         self.pool = pool
+        self._kv4 = getattr(pool, "dtype", None) == torch.uint8
         self.tp = tp
         self.is_scheduler = tp is None or tp.rank == 0
         self.leader, self.worker = (leader if self.is_scheduler else None), worker
@@ -305,6 +306,7 @@ class LLMEngine:
         is alive, so instances release their graphs before their groups go away."""
         torch.cuda.synchronize(self.device)
         self.batch.graph = None
+        self.check()
 
     def add_request(self, req: Request) -> None:
         if not self.is_scheduler:
@@ -353,7 +355,14 @@ class LLMEngine:
         self._inflight.append(ev)
         while len(self._inflight) > max(1, self.cfg.max_inflight_steps):
             self._inflight.popleft().synchronize()
+        self.check()
         return self._finished_now
+
+    def check(self) -> None:
+        """Raise if a decode step that the host has waited for failed on the device (its tokens are not to be used).
+        Every ``step`` does so; after the last one, call it once the outputs have arrived."""
+        if self._kv4:
+            kv4_ops.check_kv4_status(self.device)
 
     # ----------------------------------------------------------- schedule
     def _schedule(self) -> StepPlan:

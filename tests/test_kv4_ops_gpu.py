@@ -828,3 +828,27 @@ def test_strides_of_dimensions_of_one_do_not_matter():
     q1 = q[:, :4].contiguous()
     _check_attn(kv4_ops.paged_decode_attn_kv4(q1, one, _i32([[0]]), _i32([page]), 0.1), q1,
                 [tuple(x[:page, :1] for x in vals[0])], 0.1)
+
+
+@pytest.mark.parametrize("hkv,order", [(3, "nhd"), (2, "hnd")])
+def test_a_copy_that_is_given_up_is_reported(hkv, order):
+    """With a limit of 0 no copy is waited for: the launch lets those under way arrive and ends, its results are NaN, and
+    the host reads status 3. The next launch, with the usual limit, is right."""
+    lens, hd = [3000, 0, 700], 128
+    kv, table, vals = _filled(3, lens, hkv, hd, 16, order, seed=3)
+    q = torch.randn(3, 4 * hkv, hd, device="cuda", generator=_gen(5)).to(BF)
+    seq = _i32(lens)
+    kv4_ops.kv4_status()
+    kv4_ops.set_kv4_wait_limit_ns(0)
+    try:
+        got = kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 0.1)
+        torch.cuda.synchronize()
+    finally:
+        kv4_ops.set_kv4_wait_limit_ns(None)
+    assert kv4_ops.kv4_status(reset=False) == 3
+    assert got[0].isnan().all() and got[2].isnan().all()
+    with pytest.raises(_lib.KvbmCudaError, match="status 3"):
+        kv4_ops.check_kv4_status("cuda")
+    kv4_ops.check_kv4_status()  # cleared
+    _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 0.1), q, vals, 0.1)
+    assert kv4_ops.kv4_status() == 0

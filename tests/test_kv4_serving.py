@@ -35,3 +35,67 @@ def test_scratch_of_a_captured_step_is_kept():
     for batch in range(2, 200):
         m.decode_scratch(batch, 1)
     assert [s is mine for s in m._outgrown] == [True]
+
+
+class _Pool:
+    dtype = torch.uint8
+
+
+class _FakeModel:
+    """The engine's view of a model, on the CPU."""
+
+    device = torch.device("cpu")
+
+    class cfg:
+        kv_heads, heads, head_dim, layers = 2, 4, 64, 1
+
+    def allocate_pool(self, n, page, kv_bits=16):
+        assert kv_bits == 4
+        return _Pool()
+
+    def prefill(self, tokens, pool, ids, **kw):
+        return torch.tensor([7])
+
+    def decode_step(self, tok, pos, *a):
+        return pos.long() % 100
+
+
+def _engine(monkeypatch, **kw):
+    from test_serving_engine_cpu import FakeEvent, FakeStream
+
+    from kvbm_b200.serving import engine as E
+
+    monkeypatch.setattr(torch.cuda, "Event", FakeEvent)
+    monkeypatch.setattr(torch.cuda, "Stream", FakeStream)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda self: self)
+    monkeypatch.setattr(E.llama_ops, "decode_splits", lambda *a, **k: 1)
+    return E, E.LLMEngine(_FakeModel(), E.EngineConfig(num_gpu_blocks=8, max_num_seqs=2, max_model_len=64, max_tokens=4,
+                                                       use_graphs=False, kv_bits=4), **kw)
+
+
+def test_engine_raises_when_an_attention_launch_gave_up(monkeypatch):
+    """The status is read in every step: NaN does not go on as tokens."""
+    from kvbm_b200.ops import _lib
+
+    class Lib:
+        status = 0
+
+        def kvbm_kv4_status(self, device, reset):
+            was, self.status = self.status, 0 if reset else self.status
+            return was
+
+        kvbm_error_string = None
+
+    lib = Lib()
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    E, eng = _engine(monkeypatch)
+    eng.add_request(E.Request("a", torch.arange(5, dtype=torch.int32), max_tokens=4))
+    eng.step()
+    lib.status = 3
+    with pytest.raises(_lib.KvbmCudaError, match="status 3"):
+        eng.step()
+    eng.step()
+    lib.status = 3
+    with pytest.raises(_lib.KvbmCudaError, match="status 3"):
+        eng.check()

@@ -99,7 +99,8 @@ class EngineConfig:
     record_events: bool = True           # arrival / first-token CUDA events per request
     max_inflight_steps: int = 2          # the host runs at most this many steps ahead of the GPU
     prefix_caching: bool = False         # keep finished prompts' full blocks in G1 (LRU) and match them first
-    kv_bits: int = 16                    # 4: the engine's pool holds K/V in 4 bits (a connector's tiers then hold bytes)
+    kv_bits: int = 16                    # 4: the engine's pool holds K/V in 4 bits (a connector's tiers then hold bytes).
+                                         # A pool that is passed in is taken as it is; with 4 it has to hold bytes
 
 
 class DecodeBatch:
@@ -252,6 +253,10 @@ class LLMEngine:
                  worker: ConnectorWorker | None = None, pool: KvLayout | None = None, tp=None):
         self.model, self.cfg = model, cfg
         self.device = model.device
+        if cfg.kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, not {cfg.kv_bits}")
+        if pool is not None and cfg.kv_bits == 4 and pool.dtype != torch.uint8:
+            raise ValueError(f"kv_bits=4 with a pool of {pool.dtype}")
         if pool is None:
             bits = {} if cfg.kv_bits == 16 else {"kv_bits": cfg.kv_bits}
             pool = model.allocate_pool(cfg.num_gpu_blocks, cfg.block_size, **bits)

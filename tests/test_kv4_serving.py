@@ -99,3 +99,18 @@ def test_engine_raises_when_an_attention_launch_gave_up(monkeypatch):
     lib.status = 3
     with pytest.raises(_lib.KvbmCudaError, match="status 3"):
         eng.check()
+
+
+def test_engine_refuses_a_16_bit_pool_for_4_bits(monkeypatch):
+    from kvbm_b200.serving import engine as E
+
+    _engine(monkeypatch)
+    pool = _Pool()
+    cfg = dict(num_gpu_blocks=8, max_num_seqs=2, max_model_len=64, max_tokens=4, use_graphs=False)
+    for bits in (4, 16):  # a pool that is passed in says what it holds
+        assert E.LLMEngine(_FakeModel(), E.EngineConfig(kv_bits=bits, **cfg), pool=pool).pool is pool
+    pool.dtype = torch.bfloat16
+    with pytest.raises(ValueError, match="kv_bits"):
+        E.LLMEngine(_FakeModel(), E.EngineConfig(kv_bits=4, **cfg), pool=pool)
+    with pytest.raises(ValueError, match="kv_bits"):
+        E.LLMEngine(_FakeModel(), E.EngineConfig(kv_bits=8, **cfg), pool=pool)

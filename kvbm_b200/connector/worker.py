@@ -288,6 +288,9 @@ class ConnectorWorker:
         """
         from ..parallel.pd import HostMailbox
 
+        if wire_dtype == "fp8" and self.g1.dtype == torch.uint8:
+            raise ValueError("a pool of bytes (a 4-bit cache) goes over the wire as it is: wire_dtype fp8 is for 16-bit "
+                             "pools")
         self.instance_id, self.directory, self.push_timing = int(instance_id), directory, timing
         self.tp_rank, self.tp_size = int(tp_rank), int(tp_size)
         import os

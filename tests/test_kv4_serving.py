@@ -114,3 +114,13 @@ def test_engine_refuses_a_16_bit_pool_for_4_bits(monkeypatch):
         E.LLMEngine(_FakeModel(), E.EngineConfig(kv_bits=4, **cfg), pool=pool)
     with pytest.raises(ValueError, match="kv_bits"):
         E.LLMEngine(_FakeModel(), E.EngineConfig(kv_bits=8, **cfg), pool=pool)
+
+
+def test_fp8_on_the_wire_is_refused_for_a_pool_of_bytes():
+    """At setup, not with the first push in the middle of a request."""
+    from kvbm_b200.connector.worker import ConnectorWorker
+
+    w = object.__new__(ConnectorWorker)
+    w.g1 = _Pool()
+    with pytest.raises(ValueError, match="wire_dtype"):
+        w.enable_disagg(1, None, mailbox_slots=4, wire_dtype="fp8")

@@ -45,6 +45,7 @@ from ..engine.cd import ConditionalDisagg, InflightBudget, SelectionPolicy
 from ..engine.leader import InstanceLeader
 from ..logical.manager import BlockManager, Tier
 from ..models.llama import LlamaConfig, LlamaModel
+from ..ops.kv4_ops import row_bytes
 from ..utils.config import KvbmConfig
 from .engine import EngineConfig, LLMEngine, Request
 
@@ -67,6 +68,13 @@ class PdConfig:
     seed: int = 0
     recv_timeout_s: float = 300.0
     wire_dtype: str = "bf16"         # bf16 | fp8 (block-scaled e4m3 over NVLink, dequantised on arrival)
+    kv_bits: int = 16                # 4: both instances' pools hold K/V in 4 bits, and the push moves their bytes
+
+    def __post_init__(self) -> None:
+        if self.kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 4 or 16, not {self.kv_bits}")
+        if self.kv_bits == 4 and self.wire_dtype == "fp8":
+            raise ValueError("a 4-bit cache goes over the wire as it is: wire_dtype fp8 is for 16 bits")
 
     @property
     def request_blocks(self) -> int:
@@ -78,7 +86,8 @@ class PdConfig:
 
     def kv_bytes_per_request(self) -> int:
         c = self.model
-        return self.prompt_blocks * c.layers * 2 * self.page_size * c.kv_heads * c.head_dim * 2
+        row = row_bytes(c.head_dim) if self.kv_bits == 4 else 2 * c.head_dim
+        return self.prompt_blocks * c.layers * 2 * self.page_size * c.kv_heads * row
 
 
 class PdInstance:
@@ -118,7 +127,7 @@ class PdInstance:
         ecfg = EngineConfig(num_gpu_blocks=nblocks, block_size=bs, max_num_seqs=max_seqs,
                             max_num_batched_tokens=max(cfg.prompt_len, 2048),
                             max_model_len=cfg.prompt_len + cfg.gen_len, max_tokens=cfg.gen_len,
-                            use_graphs=cfg.use_graphs and role == "decode")
+                            use_graphs=cfg.use_graphs and role == "decode", kv_bits=cfg.kv_bits)
         self.engine = LLMEngine(model, ecfg, self.leader, self.worker, tp=tp)
         self.worker.register_layout(self.engine.pool)
         self.worker.enable_disagg(self.instance_id, directory, mailbox_slots=slots, shared=shared,

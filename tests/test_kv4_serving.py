@@ -124,3 +124,15 @@ def test_fp8_on_the_wire_is_refused_for_a_pool_of_bytes():
     w.g1 = _Pool()
     with pytest.raises(ValueError, match="wire_dtype"):
         w.enable_disagg(1, None, mailbox_slots=4, wire_dtype="fp8")
+
+
+def test_disaggregation_in_4_bits_counts_its_bytes():
+    from kvbm_b200.serving.pd import PdConfig
+
+    model = LlamaConfig(hidden=64, layers=3, heads=4, kv_heads=2, head_dim=128, intermediate=64, vocab=16)
+    a, b = PdConfig(model=model, prompt_len=40), PdConfig(model=model, prompt_len=40, kv_bits=4)
+    assert a.kv_bytes_per_request() == 3 * 3 * 2 * 16 * 2 * 256 and b.kv_bytes_per_request() == 3 * 3 * 2 * 16 * 2 * 80
+    with pytest.raises(ValueError, match="kv_bits"):
+        PdConfig(kv_bits=8)
+    with pytest.raises(ValueError, match="wire_dtype"):
+        PdConfig(kv_bits=4, wire_dtype="fp8")

@@ -260,6 +260,8 @@ class LlamaModel:
         c = self.cfg
         T = tokens.numel()
         page = pool.config.page_size
+        if start_pos + T > block_ids.numel() * page:  # their slots would be -1, and they would not be written
+            raise ValueError(f"{block_ids.numel()} blocks of {page} do not hold {start_pos} + {T} tokens")
         pos = torch.arange(start_pos, start_pos + T, device=self.device, dtype=torch.int32)
         block_ids = block_ids.to(torch.int32).contiguous()
         slots = table_ops.slot_map(block_ids, pos, page=page)

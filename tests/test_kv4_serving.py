@@ -136,3 +136,16 @@ def test_disaggregation_in_4_bits_counts_its_bytes():
         PdConfig(kv_bits=8)
     with pytest.raises(ValueError, match="wire_dtype"):
         PdConfig(kv_bits=4, wire_dtype="fp8")
+
+
+def test_prefill_refuses_too_few_blocks():
+    class Pool:
+        dtype = torch.bfloat16
+
+        class config:
+            page_size = 16
+
+    m, ids = _model(), torch.tensor([3, 1], dtype=torch.int32)
+    for start, n in ((0, 33), (30, 3), (32, 1)):
+        with pytest.raises(ValueError, match="do not hold"):
+            m.prefill(torch.zeros(n, dtype=torch.int32), Pool(), ids, start_pos=start)

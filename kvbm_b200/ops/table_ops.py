@@ -12,6 +12,8 @@ import torch
 
 from . import _lib
 
+MAX_BATCH = 8192  # requests a call of batch_tables takes (kMaxBatch of batch_tables.cu)
+
 
 class BatchTables(NamedTuple):
     block_table: torch.Tensor  # int32 [B, max_blocks], or the caller's table
@@ -59,8 +61,8 @@ def batch_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_ids
         _check(block_counts, "block_counts", torch.int32, B, dev)
     if page <= 0 or num_tokens < 0:
         raise ValueError("page must be positive and num_tokens not negative")
-    if B > _MAX_BATCH:
-        raise ValueError(f"batch_tables takes at most {_MAX_BATCH} requests, got {B}")
+    if B > MAX_BATCH:
+        raise ValueError(f"batch_tables takes at most {MAX_BATCH} requests, got {B}")
     if table is None:
         if max_blocks is None or max_blocks < 0 or rows is not None:
             raise ValueError("without a table, max_blocks is required and rows has no meaning")
@@ -85,9 +87,6 @@ def batch_tables(query_lens: torch.Tensor, context_lens: torch.Tensor, block_ids
                   rows.data_ptr() if rows is not None else None, table.shape[0], seq_lens.data_ptr(),
                   cu_query.data_ptr(), positions.data_ptr(), slots.data_ptr(), num_tokens, st)
     return BatchTables(table, seq_lens, cu_query, positions, slots)
-
-
-_MAX_BATCH = 8192  # kMaxBatch of batch_tables.cu
 
 
 def slot_map(block_table: torch.Tensor, positions: torch.Tensor, *, page: int, out: torch.Tensor | None = None,

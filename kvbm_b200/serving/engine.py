@@ -169,11 +169,15 @@ class DecodeBatch:
         ``input_token < 0`` keeps the token already in the slot (written by the caller)."""
         if not entries:
             return
-        n = len(entries)
-        dev = self.tok.device
         for e in entries:
             if len(e[1]) > self.max_blocks:
                 raise ValueError(f"{len(e[1])} blocks exceed the decode batch's {self.max_blocks}")
+        for i in range(0, len(entries), table_ops.MAX_BATCH):
+            self._enter(entries[i: i + table_ops.MAX_BATCH])
+
+    def _enter(self, entries: list[tuple[int, list[int], int, int, int]]) -> None:
+        n = len(entries)
+        dev = self.tok.device
         scal = torch.tensor([[e[2], e[3], e[3] + 1, e[4], e[0]] for e in entries], dtype=torch.int64)
         scal_d = scal.pin_memory().to(dev, non_blocking=True)
         slots_d = scal_d[:, 4]

@@ -100,3 +100,17 @@ def test_cached_prefix_is_matched():
     assert b.block_ids[:4] == a.block_ids[:4]
     for x, y in zip(before, _rows(eng.pool, b.block_ids, 64)):
         assert torch.equal(x, y)
+
+
+def test_more_requests_enter_a_decode_batch_than_one_launch_takes():
+    from types import SimpleNamespace as NS
+
+    from kvbm_b200.serving.engine import DecodeBatch
+
+    n = 8200
+    batch = DecodeBatch(NS(device=torch.device("cuda", 0)), NS(config=NS(page_size=16)), n + 3, 2, 4, 1, dummy_block=9)
+    batch.enter([(i, [i, i + 1][: 1 + i % 2], -1, i % 17, 1) for i in range(n)])
+    want = torch.tensor([[i, i + 1 if i % 2 else 9] for i in range(n)] + [[9, 9]] * 3, dtype=torch.int32)
+    assert torch.equal(batch.block_table.cpu(), want)
+    assert batch.pos.tolist() == [i % 17 for i in range(n)] + [0] * 3
+    assert batch.active.tolist() == [1] * n + [0] * 3

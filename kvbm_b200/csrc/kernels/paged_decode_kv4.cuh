@@ -41,6 +41,8 @@
 // registers or in shared memory, with all tiles.) 11 bits are enough for the others:
 // a second fp16 part would double the products with 5 to 8 heads, and an average of
 // weights so rounded is nearer than the bf16 of the result.
+// The same goes for scores above 2^12: p comes from one multiply-add with the rounded
+// m, which is off by 2^-24 of it, and s from sums that are off by about as much.
 // Products of 32 tokens are folded into fp32 accumulators, since the tensor
 // core's own accumulation truncates.
 //
@@ -68,10 +70,10 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 66.1 us = 5.2 TB/s, one of 131,072 38.0 us = 4.4 TB/s, one of 300
-// 8.0 us; each further byte costs what it costs in a copy (1.00 of it token-first,
+// 8,448 tokens 66.4 us = 5.2 TB/s, one of 131,072 38.3 us = 4.4 TB/s, one of 300
+// 7.9 us; each further byte costs what it costs in a copy (1.00 of it token-first,
 // 0.99 head-first), the rest is the start, the last round and the merge, about 11
-// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 34.0 us = 3.1 TB/s,
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 34.1 us = 3.1 TB/s,
 // where 500 instructions a tile are the bound (1.3 of a copy a further byte, as at
 // 128 with 5 to 8 heads on one). Pages that are not a multiple of 16 tokens, whose
 // rows are copied one by one, cost 1.5 to 2.1.
@@ -120,6 +122,7 @@ constexpr int kUnit = 16;       // tokens a stage of the ring holds
 constexpr int kTile = 32;       // tokens a warp takes between two updates of its accumulators
 constexpr int kMinRounds = 2;   // a CTA takes at least so many tiles a warp: below, merging costs more than it saves
 constexpr int kWhole = 6;       // requests of up to so many rounds (kStart among them) are not cut
+constexpr float kLargeScore = 4096.f;  // of log2 of p: above, fp32 products of scores are not near enough
 constexpr uint64_t kWaitNs = 1000000000ull;  // limit of a wait for a copy
 
 // ---- instructions ----------------------------------------------------------
@@ -343,13 +346,15 @@ __device__ __forceinline__ const uint8_t* row_of(const AttnParams& P, const int3
   return P.cache.base + id * P.cache.block_stride +
          P.cache.page_div.mod(static_cast<uint32_t>(t), col) * P.cache.token_stride + kvh * P.cache.head_stride;
 }
-// Whether a group that any head lacks a large weight for has elements that differ, in any of a warp's tokens (groups of
-// equal elements, as in padding, take no weights; with one such group in four 105 us in place of 75).
+// Whether a warp's tiles are to be done again: scores are large, or a group that a head lacks a large weight for has
+// elements that differ in some token (groups of equal elements, as in padding, take no weights; with one such group in
+// four 105 us in place of 75).
 template <int HD, bool PAIR>
-__device__ __forceinline__ bool any_scale(const AttnParams& P, int b, int kvh, int seq, int t_begin, int tiles,
+__device__ __forceinline__ bool do_again(const AttnParams& P, int b, int kvh, int seq, int t_begin, int tiles,
                                           int round_tokens, uint32_t lacking) {
   constexpr int NG = HD / kGroup;
   lacking = __reduce_or_sync(0xffffffffu, lacking);
+  if (lacking & 1u) return true;
   const int32_t* table = P.table + b * P.table_stride;
   bool found = false;
   for (int tile = 0; tile < tiles; ++tile) {
@@ -639,7 +644,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
       const int e = max(exponent(top), -100);  // the largest element comes to [2^13, 2^14)
       const float up = flag ? 0.f : copysignf(pow2(13 - e), P.qscale);  // a negative scale turns q: factor is positive
       float fac = flag ? __uint_as_float(0x7fc00000u) : ldexpf(fabsf(P.qscale), 24 + e - 13);
-      if (fac < 1e-36f) fac = 1e-36f;  // (times -infinity is to be -infinity)
+      if (fac < 1e-36f) fac = 1e-36f;  // (times -infinity is to be -infinity, and times 0 to be 0)
+      if (fac > 3.4e38f) fac = 3.4e38f;
       float qs[NG];
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -689,7 +695,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     float m[NH], ref[NH], l[NH], z[NH][NG];  // ref = m factor, 0 before there is an m
     float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24; odd i: that of i - 1 and 16 times i's
     float vf = pow2(100);  // f; the first tile sets it
-    uint32_t lacking = 0u;         // the lane's heads' groups that have not been given a large weight where they should
+    uint32_t lacking = 0u;         // the lane's heads' groups that have not been given a large weight where they should;
+                                   // bit 0: scores too large for this loop
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       m[n] = -INFINITY;
@@ -976,8 +983,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           acc[g][i][n] = fmaf(acc[g][i][n] * 16777216.f, 1.f / vf, z[n][g]);
         }
     }
+    // (m large and negative at first, and higher later, has left an infinite l or a NaN, or nothing)
+#pragma unroll
+    for (int n = 0; n < NH; ++n)
+      if (fabsf(ref[n]) > kLargeScore || !(l[n] < INFINITY)) lacking |= 1u;
     if (__any_sync(0xffffffffu, lacking != 0u) && !given_up &&
-        any_scale<HD, PAIR>(P, b, kvh, seq, t_begin, mine, round_tokens, lacking))
+        do_again<HD, PAIR>(P, b, kvh, seq, t_begin, mine, round_tokens, lacking))
       share_in_fp32<HD, NH>(P, b, kvh, head0, heads, seq, t_begin, mine, round_tokens, m, l, acc);
     // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
     if (P.streams > 1) {

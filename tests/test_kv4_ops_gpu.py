@@ -852,3 +852,36 @@ def test_a_copy_that_is_given_up_is_reported(hkv, order):
     kv4_ops.check_kv4_status()  # cleared
     _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, seq, 0.1), q, vals, 0.1)
     assert kv4_ops.kv4_status() == 0
+
+
+@pytest.mark.parametrize("exponent", [10, 14, 24, 32, 60, 125])
+@pytest.mark.parametrize("group,hd", [(4, 128), (7, 64), (3, 256)])
+def test_attention_large_scores(group, hd, exponent):
+    """Scores of up to 1e38 are finite, and beside those of other tokens: all the weight lies on the largest ones."""
+    n, heads = 50, 2
+    x = torch.randn(n, 2, heads, hd, device="cuda", generator=_gen(8))
+    x[:, 0, :, 0] = torch.linspace(-1, 2, n, device="cuda")[torch.randperm(n, device="cuda", generator=_gen(9)), None]
+    kv, table, vals, _ = _held(x.to(BF))
+    q = torch.zeros(1, heads * group, hd, dtype=BF, device="cuda")
+    q[..., 0] = 2.0 ** exponent
+    q[0, 1, 0] = -(2.0 ** exponent)
+    q[0, 2, 0] = 2.0 ** (exponent - 6)
+    for ctas in (1, 2):
+        _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, ctas=ctas), q, vals, 1.0)
+
+
+@pytest.mark.parametrize("group,hd", [(4, 128), (7, 64)])
+def test_attention_large_negative_scores_in_front(group, hd):
+    """A tile whose scores are far below zero leaves nothing behind when ordinary ones follow."""
+    n, heads = 100, 2
+    x = torch.randn(n, 2, heads, hd, device="cuda", generator=_gen(8))
+    x[:, 0] = 0.0
+    x[:64, 0, :, 0] = -torch.linspace(1, 2, 64, device="cuda")[:, None]
+    x[64:, 0, :, 1] = torch.randn(36, heads, device="cuda", generator=_gen(9))
+    kv, table, vals, _ = _held(x.to(BF))
+    q = torch.zeros(1, heads * group, hd, dtype=BF, device="cuda")
+    q[..., 1] = 1.0
+    for e in (8, 20, 40, 100):
+        q[..., 0] = 2.0 ** e
+        for ctas in (1, 2):
+            _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, ctas=ctas), q, vals, 1.0)

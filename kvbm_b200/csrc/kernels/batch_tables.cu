@@ -203,9 +203,9 @@ extern "C" int kvbm_batch_tables(const int32_t* query_lens, const int32_t* conte
                                                static_cast<int>(2 * sizeof(int64_t) * (kMaxBatch + 1)));
     if (e != cudaSuccess) return e;
   }
-  // a row or 256 tokens a CTA, up to four CTAs on each of 148 SMs
+  // a row or 256 tokens a CTA, up to four CTAs on each SM
   const int64_t ctas = std::max<int64_t>(table ? batch : 0, (tokens + kThreads - 1) / kThreads);
-  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ctas, 4 * 148)));
+  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(ctas, 4 * kvbm_sm_count())));
   batch_tables_kernel<<<grid, kThreads, smem, stream>>>(P);
   return cudaGetLastError();
 }

@@ -26,18 +26,20 @@ constexpr int kReadThreads = 128;
 //   out[i] = y[i] cos - y[i + R/2] sin, out[i + R/2] = y[i + R/2] cos + y[i] sin,  i < R/2; the rest as it is
 //
 // all in fp32 and rounded to bf16 once. The cache takes that bf16 k and the bf16
-// v, so quantising a 16-bit cache later gives the same codes.
+// v, so quantising a 16-bit cache that this kernel has written gives the same codes.
+// (The 16-bit write of models without head norms, rope_kv_write, fuses a product and
+// a sum of the rotation: its k may be a bf16 step away, and a code with it.)
 //
 // A row of HD elements is held by HD/16 lanes, each with 8 elements of the first
 // half and the 8 that lie HD/2 behind them, so with rot = HD both elements of a
 // rotation are in one lane (with a smaller rot the other comes by shuffle), and
 // a warp takes 512 / HD rows a step. Every product is rounded to fp32 by itself in
-// the order of the formula, and the squares are summed in the order of an unfused
-// evaluation (sum_squares), so that k's bf16 values, and with them the codes of a
-// 4-bit cache, do not depend on which of the two computed them: one fp32 step
-// moves a code that lies next to a border by a fifteenth of its group's range
-// (folding w into cos and sin, two of five products less an element, moved 4 codes
-// in a chunk of 8,192 tokens).
+// the order of the formula, and the squares are summed in the order in which PyTorch's
+// reductions sum a row (sum_squares). Nothing else in this library computes k so: it
+// makes k, and the codes, the same bit for bit as the formula's operations one after
+// another, which is how they are checked, where one fp32 step moves a code that lies
+// next to a border by a fifteenth of its group's range (folding w into cos and sin,
+// two of five products less an element, moved 4 codes in a chunk of 8,192 tokens).
 // What bounds it is HBM for a prefill (the rows go in and out once), nearly
 // matched by the instructions of the norm, the rotation and the quantising (250 a
 // step; at the HBM rate an SM issues 340): hence the packed arithmetic, and copies
@@ -469,7 +471,8 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   // tokens alone take all places (2,048 tokens of 32 + 16 heads of 128: whole tokens 13.6 us, two warps a token, of
   // which the last ones wait for a place, 16.0; 512 tokens: six warps a token 5.1, four 5.6).
   const int steps = P.steps_q + 2 * P.steps_kv;
-  const int64_t items = std::clamp<int64_t>(148 * write_warps_sm(rot == hd) / tokens, 1, steps);
+  const int64_t places = static_cast<int64_t>(kvbm_sm_count()) * write_warps_sm(rot == hd);
+  const int64_t items = std::clamp<int64_t>(places / tokens, 1, steps);
   P.steps_item = static_cast<int>((steps + items - 1) / items);
   P.items_div = FastDiv(static_cast<uint32_t>((steps + P.steps_item - 1) / P.steps_item));
   const int64_t warps = tokens * P.items_div.d;
@@ -477,7 +480,7 @@ extern "C" int kvbm_qk_norm_rope_kv_write(void* qkv, int64_t qkv_stride, int64_t
   // The next kernel (a decode step's attention) is let in early only where this one leaves most places free: 3 us a
   // layer of a decode step of 32 requests; filling the places beside 200 tokens' 2,400 warps cost 0.3 us, since the
   // blocks that found none were placed unevenly.
-  P.release = warps * 4 <= 148 * write_warps_sm(rot == hd);
+  P.release = warps * 4 <= places;
   const unsigned grid = static_cast<unsigned>((warps + kWriteThreads / 32 - 1) / (kWriteThreads / 32));
 #define KVBM_WRITE(HD, KV4, FULL) \
   kv4::launch_overlapped(qk_norm_rope_kv_write_kernel<HD, KV4, FULL>, dim3(grid), kWriteThreads, 0, stream, P)

@@ -1061,11 +1061,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 
 // How a launch is laid out: (KV head, chunk) pairs and streams a CTA, CTAs along the work.
 struct Plan {
-  int chunks, y_total, y_cta, y_ctas, streams, ctas;
+  int chunks, y_total, y_cta, y_ctas, streams, ctas, sms;
   bool cut;  // whether a request may be cut, and the merge is to follow
 };
 inline Plan plan_decode(int batch, int hq, int hkv, int hd, int64_t max_tokens, int ctas, int sm_count) {
   Plan p{};
+  p.sms = sm_count;
   p.chunks = (hq / hkv + kHeads - 1) / kHeads;
   p.y_total = hkv * p.chunks;
   // Where requests are short and few, one KV head a CTA: its 8 streams of tokens take a request's 1,024 tokens in 4
@@ -1177,7 +1178,7 @@ cudaError_t launch_decode_hd(AttnParams& P, const Plan& plan, cudaStream_t strea
                    : launch_decode_kernel<HD, false, kTma>(P, map, plan, stream);
   }
   if (e != cudaSuccess || !plan.cut) return e;
-  const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 2 * 148 ? 1 : kMergeWarps;
+  const int heads_cta = static_cast<int64_t>(P.batch) * P.hq <= 2 * plan.sms ? 1 : kMergeWarps;
   return launch_overlapped(kv4_merge_kernel<HD>, dim3((P.hq + heads_cta - 1) / heads_cta, P.batch), kMergeWarps * 32, 0,
                            stream, P, heads_cta);
 }

@@ -70,10 +70,10 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 66.4 us = 5.2 TB/s, one of 131,072 38.3 us = 4.4 TB/s, one of 300
+// 8,448 tokens 66.3 us = 5.2 TB/s, one of 131,072 38.2 us = 4.4 TB/s, one of 300
 // 7.9 us; each further byte costs what it costs in a copy (1.00 of it token-first,
 // 0.99 head-first), the rest is the start, the last round and the merge, about 11
-// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 34.1 us = 3.1 TB/s,
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.8 us = 3.1 TB/s,
 // where 500 instructions a tile are the bound (1.3 of a copy a further byte, as at
 // 128 with 5 to 8 heads on one). Pages that are not a multiple of 16 tokens, whose
 // rows are copied one by one, cost 1.5 to 2.1.
@@ -346,15 +346,12 @@ __device__ __forceinline__ const uint8_t* row_of(const AttnParams& P, const int3
   return P.cache.base + id * P.cache.block_stride +
          P.cache.page_div.mod(static_cast<uint32_t>(t), col) * P.cache.token_stride + kvh * P.cache.head_stride;
 }
-// Whether a warp's tiles are to be done again: scores are large, or a group that a head lacks a large weight for has
-// elements that differ in some token (groups of equal elements, as in padding, take no weights; with one such group in
-// four 105 us in place of 75).
-template <int HD, bool PAIR>
-__device__ __forceinline__ bool do_again(const AttnParams& P, int b, int kvh, int seq, int t_begin, int tiles,
-                                          int round_tokens, uint32_t lacking) {
+// Whether one of the groups (a bit each) has elements that differ in one of a warp's tokens: groups of equal elements, as
+// in padding, take no weights (with one such group in four 105 us in place of 75).
+template <int HD>
+__device__ __forceinline__ bool any_scale(const AttnParams& P, int b, int kvh, int seq, int t_begin, int tiles,
+                                          int round_tokens, uint32_t groups) {
   constexpr int NG = HD / kGroup;
-  lacking = __reduce_or_sync(0xffffffffu, lacking);
-  if (lacking & 1u) return true;
   const int32_t* table = P.table + b * P.table_stride;
   bool found = false;
   for (int tile = 0; tile < tiles; ++tile) {
@@ -362,8 +359,7 @@ __device__ __forceinline__ bool do_again(const AttnParams& P, int b, int kvh, in
     const uint8_t* k = t < seq ? row_of(P, table, t, kvh) : nullptr;
     if (k == nullptr) continue;
     for (int g = 0; g < NG; ++g) {
-      const uint32_t mine = PAIR ? (g & 1 ? 0x40000000u : 0x4000u) >> (g / 2) : 0x40004000u >> g;
-      if (lacking & mine)
+      if ((groups >> g) & 1u)
         found |= (*reinterpret_cast<const uint32_t*>(k + P.cache.outer_stride + HD / 2 + 4 * g) & 0xffffu) != 0u;
     }
   }
@@ -695,8 +691,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     float m[NH], ref[NH], l[NH], z[NH][NG];  // ref = m factor, 0 before there is an m
     float acc[NG][4][NH];  // element 32 g + 4 gid + i, times f 2^-24; odd i: that of i - 1 and 16 times i's
     float vf = pow2(100);  // f; the first tile sets it
-    uint32_t lacking = 0u;         // the lane's heads' groups that have not been given a large weight where they should;
-                                   // bit 0: scores too large for this loop
+    constexpr int kWords = (NB + 3) / 4;
+    uint32_t lacking[kWords] = {};         // the lane's heads' groups that have not been given a large weight where they should
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
       m[n] = -INFINITY;
@@ -892,15 +888,22 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
         for (int n = 0; n < NH; ++n) alpha[n] *= pow2(max(now - old, -126));
       }
-      if (higher || set) {  // has each group been given a weight of 2 or more, bit 14 of an fp16?
-        constexpr uint32_t kLow = 0x4000u / (1u << (NB - 1)) * ((1u << NB) - 1u);  // operand k: bits 14 - k, 30 - k
-        uint32_t have = (alpha[0] == 1.f ? kLow : 0u) | (alpha[NH - 1] == 1.f ? kLow << 16 : 0u);
+      if (higher || set) {  // has each group that needs it been given a weight of 2 or more, bit 14 of an fp16?
+        // operand k of lanes tig at bits 15 - (4 tig + k) and 16 above, four operands a word
+        constexpr int kOps = NB < 4 ? NB : 4;
+        constexpr uint32_t kMine = 0x8000u / (1u << (kOps - 1)) * ((1u << kOps) - 1u);
+        constexpr uint32_t kAll = (kMine | kMine >> 4 | kMine >> 8 | kMine >> 12) * 0x10001u;
+        const uint32_t own = (kMine >> (4 * tig)) * 0x10001u;
+        const uint32_t exempt = (alpha[0] == 1.f ? own & 0xffffu : 0u) | (alpha[NH - 1] == 1.f ? own & 0xffff0000u : 0u);
 #pragma unroll
-        for (int k = 0; k < NB; ++k)
-          have |= ((bp[0][k][0] | bp[0][k][1] | bp[1][k][0] | bp[1][k][1]) & 0x40004000u) >> k;
+        for (int w = 0; w < kWords; ++w) {
+          uint32_t have = 0u;
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) have |= __shfl_xor_sync(0xffffffffu, have, o);
-        lacking |= (kLow | kLow << 16) & ~have;
+          for (int k = 4 * w; k < 4 * w + kOps; ++k)
+            have |= ((bp[0][k][0] | bp[0][k][1] | bp[1][k][0] | bp[1][k][1]) & 0x40004000u) >> (k & 3);
+          have = __reduce_or_sync(0xffffffffu, ((have << 1) >> (4 * tig)) | exempt);
+          lacking[w] |= kAll & ~have;
+        }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -983,12 +986,21 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
           acc[g][i][n] = fmaf(acc[g][i][n] * 16777216.f, 1.f / vf, z[n][g]);
         }
     }
-    // (m large and negative at first, and higher later, has left an infinite l or a NaN, or nothing)
+    bool large = false;  // (m large and negative at first, and higher later, has left an infinite l or a NaN, or nothing)
 #pragma unroll
     for (int n = 0; n < NH; ++n)
-      if (fabsf(ref[n]) > kLargeScore || !(l[n] < INFINITY)) lacking |= 1u;
-    if (__any_sync(0xffffffffu, lacking != 0u) && !given_up &&
-        do_again<HD, PAIR>(P, b, kvh, seq, t_begin, mine, round_tokens, lacking))
+      large |= fabsf(ref[n]) > kLargeScore || !(l[n] < INFINITY);
+    uint32_t groups = 0u;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w)
+#pragma unroll
+      for (int k = 4 * w; k < 4 * w + 4 && k < NB; ++k) {
+        if (lacking[w] & (0x8888u >> (k & 3))) groups |= 1u << (PAIR ? 2 * k : k);
+        if (lacking[w] & (0x88880000u >> (k & 3))) groups |= 1u << (PAIR ? 2 * k + 1 : k);
+      }
+    large = __any_sync(0xffffffffu, large);
+    if ((large || groups != 0u) && !given_up &&
+        (large || any_scale<HD>(P, b, kvh, seq, t_begin, mine, round_tokens, groups)))
       share_in_fp32<HD, NH>(P, b, kvh, head0, heads, seq, t_begin, mine, round_tokens, m, l, acc);
     // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
     if (P.streams > 1) {

@@ -70,13 +70,13 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 66.3 us = 5.2 TB/s, one of 131,072 38.2 us = 4.4 TB/s, one of 300
-// 7.9 us; each further byte costs what it costs in a copy (1.00 of it token-first,
-// 0.99 head-first), the rest is the start, the last round and the merge, about 11
-// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.8 us = 3.1 TB/s,
-// where 500 instructions a tile are the bound (1.3 of a copy a further byte, as at
+// 8,448 tokens 66.3 us = 5.2 TB/s, one of 131,072 38.1 us = 4.4 TB/s, one of 300
+// 7.9 us; each further byte costs what it costs in a copy (1.03 of it token-first,
+// 1.02 head-first), the rest is the start, the last round and the merge, about 11
+// us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.9 us = 3.1 TB/s,
+// where 520 instructions a tile are the bound (1.3 of a copy a further byte, as at
 // 128 with 5 to 8 heads on one). Pages that are not a multiple of 16 tokens, whose
-// rows are copied one by one, cost 1.5 to 2.1.
+// rows are copied one by one, cost 1.6 to 1.8.
 #pragma once
 
 #include "common.cuh"

@@ -70,7 +70,7 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 66.3 us = 5.2 TB/s, one of 131,072 38.1 us = 4.4 TB/s, one of 300
+// 8,448 tokens 66.5 us = 5.2 TB/s, one of 131,072 38.1 us = 4.4 TB/s, one of 300
 // 7.9 us; each further byte costs what it costs in a copy (1.03 of it token-first,
 // 1.02 head-first), the rest is the start, the last round and the merge, about 11
 // us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.9 us = 3.1 TB/s,
@@ -1002,6 +1002,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
     if ((large || groups != 0u) && !given_up &&
         (large || any_scale<HD>(P, b, kvh, seq, t_begin, mine, round_tokens, groups)))
       share_in_fp32<HD, NH>(P, b, kvh, head0, heads, seq, t_begin, mine, round_tokens, m, l, acc);
+    if constexpr (SHARED) give_back();  // a warp's limited waits are for copies, not for the other's second go
     // ---- streams of this CTA: the first one's warp takes the others' results, lane by lane
     if (P.streams > 1) {
       constexpr int kVals = NH * (2 + 4 * NG);

@@ -885,3 +885,24 @@ def test_attention_large_negative_scores_in_front(group, hd):
         q[..., 0] = 2.0 ** e
         for ctas in (1, 2):
             _check_attn(kv4_ops.paged_decode_attn_kv4(q, kv, table, _i32([n]), 1.0, ctas=ctas), q, vals, 1.0)
+
+
+def test_attention_a_warp_that_starts_again_keeps_no_other_waiting():
+    """Two warps share the copies of two heads. One of them does its tiles again in fp32, for milliseconds: the other's
+    wait for the next request's copies, which the first issues, begins when that is done."""
+    n, hd = 3000, 128
+    x = torch.randn(n, 2, 8, hd, device="cuda", generator=_gen(3))
+    x[:, 1, 0, :32] *= 1e6  # the first head's
+    kv, table, vals, _ = _held(x.to(BF))
+    q = torch.randn(1, 16, hd, device="cuda", generator=_gen(4)).to(BF)
+    kv4_ops.kv4_status()
+    kv4_ops.set_kv4_wait_limit_ns(1_000_000)
+    try:
+        got = kv4_ops.paged_decode_attn_kv4(q.expand(3, 16, hd).contiguous(), kv, table.expand(3, -1).contiguous(),
+                                            _i32([n] * 3), 0.1, ctas=1)
+        torch.cuda.synchronize()
+    finally:
+        kv4_ops.set_kv4_wait_limit_ns(None)
+    assert kv4_ops.kv4_status() == 0
+    for row in got:
+        _check_attn(row[None], q, vals, 0.1)

@@ -70,7 +70,7 @@
 // barrier of the two where a tile's stage is given back.
 //
 // Measured, pages of 16 tokens, heads of 128, 32 on 8 KV heads: 32 requests of
-// 8,448 tokens 66.5 us = 5.2 TB/s, one of 131,072 38.1 us = 4.4 TB/s, one of 300
+// 8,448 tokens 65.6 us = 5.3 TB/s, one of 131,072 38.0 us = 4.4 TB/s, one of 300
 // 7.9 us; each further byte costs what it costs in a copy (1.03 of it token-first,
 // 1.02 head-first), the rest is the start, the last round and the merge, about 11
 // us. Heads of 64, 28 on 4: 61 requests of up to 9,000 tokens 33.9 us = 3.1 TB/s,
@@ -893,7 +893,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
         constexpr int kOps = NB < 4 ? NB : 4;
         constexpr uint32_t kMine = 0x8000u / (1u << (kOps - 1)) * ((1u << kOps) - 1u);
         constexpr uint32_t kAll = (kMine | kMine >> 4 | kMine >> 8 | kMine >> 12) * 0x10001u;
-        const uint32_t own = (kMine >> (4 * tig)) * 0x10001u;
+        // (from 128 on made anew each time: 1.3 % with 4 heads of 128; at 64 kept in registers, there are some: 1.3 %)
+        const uint32_t at = 4 * (HD < 128 ? tig : seldom(tig)), own = (kMine >> at) * 0x10001u;
         const uint32_t exempt = (alpha[0] == 1.f ? own & 0xffffu : 0u) | (alpha[NH - 1] == 1.f ? own & 0xffff0000u : 0u);
 #pragma unroll
         for (int w = 0; w < kWords; ++w) {
@@ -901,7 +902,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Geometry<HD>::kCtasPerSm)
 #pragma unroll
           for (int k = 4 * w; k < 4 * w + kOps; ++k)
             have |= ((bp[0][k][0] | bp[0][k][1] | bp[1][k][0] | bp[1][k][1]) & 0x40004000u) >> (k & 3);
-          have = __reduce_or_sync(0xffffffffu, ((have << 1) >> (4 * tig)) | exempt);
+          have = __reduce_or_sync(0xffffffffu, ((have << 1) >> at) | exempt);
           lacking[w] |= kAll & ~have;
         }
       }

@@ -28,7 +28,7 @@ import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 from torch.nn.attention.bias import causal_lower_right
 
-from ..ops import kv4_ops, llama_ops, table_ops
+from ..ops import _lib, kv4_ops, llama_ops, table_ops
 from ..physical.layout import KvBlockLayout, KvLayout, LayoutConfig
 
 
@@ -214,6 +214,7 @@ class LlamaModel:
         self._scratch_stream: torch.cuda.Stream | None = None
         self._outgrown: list[torch.Tensor] = []  # earlier ones that captured steps go on using
         self._decode_counters: torch.Tensor | None = None
+        self._counters_captured = False
         self.decode_gemm = "cublas"  # "tc": decode projections on the tcgen05 skinny GEMM
         self._gemm_ws: llama_ops.GemmWorkspace | None = None
         self._attn_backends: dict[bool, list] = {}
@@ -366,14 +367,17 @@ class LlamaModel:
         return self._scratch(batch * self.cfg.heads * splits * (self.cfg.head_dim + 2))
 
     def _capturing(self) -> bool:
-        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        return _lib.capturing(self.device)
 
     def _scratch(self, need: int) -> torch.Tensor:
         """``need`` floats that the decode steps share. It grows by half at least, so that a batch that grows by one
-        request at a time does not make one for each; an outgrown one is kept only if a captured step was given it."""
+        request at a time does not make one for each; an outgrown one is kept only if a captured step was given it.
+        A step under capture that needs more than there is gets one of its own, in the graph's memory."""
         have = 0 if self._decode_scratch is None else self._decode_scratch.numel()
         capturing = self._capturing()
         if self._decode_scratch is None or have < need:
+            if capturing:
+                return torch.empty(need, dtype=torch.float32, device=self.device)
             if self._scratch_captured:
                 self._outgrown.append(self._decode_scratch)
             self._decode_scratch = torch.empty(max(need, have + have // 2), dtype=torch.float32, device=self.device)
@@ -396,10 +400,18 @@ class LlamaModel:
         return F.linear(x, w)
 
     def decode_counters(self, batch: int) -> torch.Tensor:
-        """Zeroed split-merge tickets for the attention kernel (it leaves them zero after every launch)."""
+        """Zeroed split-merge tickets for the attention kernel (it leaves them zero after every launch). Those that a
+        captured step was given are kept; a capture that needs more than there are zeroes its own at every replay."""
         need = batch * self.cfg.kv_heads
+        capturing = self._capturing()
         if self._decode_counters is None or self._decode_counters.numel() < need:
-            self._decode_counters = torch.zeros(need, dtype=torch.int32, device=self.device)
+            made = torch.zeros(need, dtype=torch.int32, device=self.device)
+            if capturing:
+                return made
+            if self._counters_captured:
+                self._outgrown.append(self._decode_counters)
+            self._decode_counters, self._counters_captured = made, False
+        self._counters_captured |= capturing
         return self._decode_counters
 
     @torch.inference_mode()

@@ -249,6 +249,11 @@ def call(name: str, *args) -> None:
     count_launches(_KERNELS_PER_CALL.get(name, 0))
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether the current stream is being captured into a graph."""
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class on_device:
     """Makes ``device`` current and, given a stream (``torch.cuda.Stream`` or handle), that stream: what is
     allocated inside belongs to the stream the kernel runs on. Yields the stream's handle."""

@@ -12,6 +12,7 @@ def _model():
     m.cfg = LlamaConfig(hidden=64, layers=1, heads=2, kv_heads=1, head_dim=64, intermediate=64, vocab=16)
     m.device = torch.device("cpu")
     m._decode_scratch, m._outgrown, m._scratch_captured, m._scratch_stream = None, [], False, None
+    m._decode_counters, m._counters_captured = None, False
     return m
 
 

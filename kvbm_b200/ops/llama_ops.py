@@ -150,18 +150,31 @@ class GemmWorkspace:
     kernel re-zeroes what it used).
 
     One workspace serves launches that run one after another; GEMMs that may run
-    at the same time (different streams) need one each."""
+    at the same time (different streams) need one each. Buffers that a captured
+    launch was given are kept when a larger GEMM outgrows them; a launch under
+    capture that needs more than there is zeroes its own at every replay."""
 
     def __init__(self, device, elems: int = 0, tiles: int = 0):
         self.device = torch.device(device)
         self.ws = torch.zeros(max(elems, 1), dtype=torch.float32, device=self.device)
         self.tickets = torch.zeros(max(tiles, 1), dtype=torch.int32, device=self.device)
 
-    def reserve(self, elems: int, tiles: int) -> None:
-        if self.ws.numel() < elems:
-            self.ws = torch.zeros(elems, dtype=torch.float32, device=self.device)
-        if self.tickets.numel() < tiles:
-            self.tickets = torch.zeros(tiles, dtype=torch.int32, device=self.device)
+        self._captured = False
+        self._kept: list[torch.Tensor] = []
+
+    def reserve(self, elems: int, tiles: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Sums and tickets for a launch of this size."""
+        capturing = _lib.capturing(self.device)
+        if self.ws.numel() < elems or self.tickets.numel() < tiles:
+            made = (torch.zeros(max(elems, self.ws.numel()), dtype=torch.float32, device=self.device),
+                    torch.zeros(max(tiles, self.tickets.numel()), dtype=torch.int32, device=self.device))
+            if capturing:
+                return made
+            if self._captured:
+                self._kept += [self.ws, self.tickets]
+            (self.ws, self.tickets), self._captured = made, False
+        self._captured |= capturing
+        return self.ws, self.tickets
 
     def clear(self) -> None:
         """Zero the partial sums and tickets (after a launch that gave up: an aborted CTA
@@ -199,9 +212,9 @@ def skinny_gemm(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = Non
         workspace = _workspaces.get(dev)
         if workspace is None:
             workspace = _workspaces[dev] = GemmWorkspace(x.device)
-    workspace.reserve(M * N, -(-N // 128))
+    ws, tickets = workspace.reserve(M * N, -(-N // 128))
     _lib.call("kvbm_skinny_gemm", x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), out.data_ptr(),
-              out.stride(0), M, N, K, int(ctas), workspace.ws.data_ptr(), workspace.tickets.data_ptr(),
+              out.stride(0), M, N, K, int(ctas), ws.data_ptr(), tickets.data_ptr(),
               _stream(stream))
     return out
 
